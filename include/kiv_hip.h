@@ -323,6 +323,110 @@ int kiv_prefill_attention(const kiv_attention_args_t *args, kiv_stream_t stream)
 size_t kiv_prefill_workspace_size(int32_t batch, int32_t num_q_heads, int32_t head_dim, int32_t q_len,
                                   int32_t cold_len, int32_t hot_len);
 
+/* ---- Paged cache: sequences of different lengths (no counterpart in the reference) ----
+ *
+ * A pool of pages of page_size tokens holds K and V rows of many sequences;
+ * a block table gives each sequence's pages.  New tokens of all sequences
+ * are packed one behind the other (sequence b's are rows cu_q[b] ..
+ * cu_q[b + 1] - 1).  kiv_paged_append writes their K and V rows to their
+ * pages, with the head norms and the position rotation applied on the way;
+ * kiv_paged_attention attends over the pages.  kiv_norm_rope is the norm
+ * and rotation alone, for rows that stay where the caller keeps them (the
+ * tiered cache's hot window, say).
+ *
+ * Lengths and tables are read on the device only: no call synchronises, and
+ * a captured call follows what the arrays hold at each replay.  Whatever
+ * they hold, no row outside the pool, the packed rows and the outputs is
+ * read or written: a table entry outside [0, num_pages) is a page that is
+ * not there (appends to it are dropped, its keys are not seen). */
+
+/* Position rotation: entry pair i (i < rot_dim / 2) of a row turns by
+ * position * inv_freq[i] and is scaled by `scale`.  Pair i is entries i and
+ * i + rot_dim / 2, or with `interleaved` entries 2 i and 2 i + 1; entries
+ * from rot_dim on stay.  Angles are formed in 64 bits. */
+typedef struct {
+  const float *inv_freq;      /* [rot_dim / 2] */
+  const int32_t *axes;        /* [rot_dim / 2] position axis of each pair, or NULL: axis 0 */
+  const void *positions;      /* int32 or int64; NULL (paged append only): the token's key index */
+  int64_t position_stride[3]; /* axis, b, t (elements; 0 broadcasts) */
+  int32_t position_bytes;     /* 4 or 8 */
+  int32_t num_axes;           /* axes of `positions`, >= 1 */
+  int32_t rot_dim;            /* 0: no rotation; a multiple of 16 (fp32: 8), at most head_dim */
+  int32_t interleaved;
+  float scale;                /* of the cosines and sines (1: none) */
+  int32_t _pad;
+} kiv_rotary_t;
+
+/* Norm of a head row before its rotation: x / sqrt(mean(x^2) + eps) * weight,
+ * in fp32. */
+typedef struct {
+  const float *weight; /* [head_dim] fp32, or NULL: 1 */
+  float eps;
+  int32_t enabled;     /* 0: no norm */
+} kiv_head_norm_t;
+
+/* Rows of q and k: [B, H, T, D], strides b, h, t in elements, 16-byte aligned.
+ * Outputs may be the inputs themselves (same pointer and strides). */
+typedef struct {
+  int32_t batch, tokens, num_q_heads, num_kv_heads, head_dim, dtype;
+  const void *q;
+  int64_t q_stride[3];
+  void *q_out;
+  int64_t q_out_stride[3];
+  const void *k;       /* NULL with num_kv_heads 0: q alone */
+  int64_t k_stride[3];
+  void *k_out;
+  int64_t k_out_stride[3];
+  kiv_rotary_t rotary;
+  kiv_head_norm_t q_norm, k_norm;
+} kiv_norm_rope_args_t;
+
+/* Head norms and position rotation in one pass, rounded once to the dtype.
+ * head_dim: a multiple of 8 (fp32: 4), at most 512. */
+int kiv_norm_rope(const kiv_norm_rope_args_t *args, kiv_stream_t stream);
+
+/* A pool of pages.  K and V have the same strides. */
+typedef struct {
+  void *k, *v;           /* K and V rows, 16-byte aligned */
+  int64_t stride[3];     /* page, head, token (elements) */
+  int32_t num_pages, page_size, num_kv_heads, head_dim, dtype, _pad;
+} kiv_paged_cache_t;
+
+/* A ragged batch of new tokens over the pool (device arrays). */
+typedef struct {
+  const int32_t *cu_q;        /* [num_seqs + 1] first packed row of each sequence; rows from the last on are
+                                 no sequence's: left as they are */
+  const int32_t *kv_len;      /* [num_seqs] keys, the new tokens' among them: packed row r of sequence b has
+                                 key index kv_len[b] - cu_q[b + 1] + r */
+  const int32_t *block_table; /* [num_seqs, table_width] pages; row stride table_stride (elements) */
+  int64_t table_stride;
+  int32_t num_seqs, table_width, total_q; /* total_q: packed rows */
+  int32_t max_q_len, max_kv_len;          /* bounds of the lengths (they choose the kernel only: wrong ones cost
+                                             time, not results) */
+  int32_t _pad;
+} kiv_paged_batch_t;
+
+typedef struct {
+  kiv_paged_cache_t cache;
+  kiv_paged_batch_t batch;
+  const void *k;         /* [total_q, Hkv, D], strides t, h */
+  int64_t k_stride[2];
+  const void *v;         /* [total_q, Hkv, D] */
+  int64_t v_stride[2];
+  const void *q;         /* [total_q, Hq, D] to be normed and rotated into q_out, or NULL with num_q_heads 0 */
+  int64_t q_stride[2];
+  void *q_out;           /* may be q */
+  int64_t q_out_stride[2];
+  int32_t num_q_heads, _pad;
+  kiv_rotary_t rotary;   /* position_stride[1] is not used */
+  kiv_head_norm_t q_norm, k_norm, v_norm;
+} kiv_paged_append_args_t;
+
+/* Writes the new tokens' K (normed, rotated) and V (normed) rows to their
+ * pages, and q beside them.  Pages named twice by the table get the rows of
+ * one of their sequences. */
+int kiv_paged_append(const kiv_paged_append_args_t *args, kiv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

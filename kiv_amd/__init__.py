@@ -3,7 +3,9 @@
 Same import surface as the reference package ``kiv`` (kiv/__init__.py:5-35):
 ``KIVConfig``, ``ColdKVStore`` and ``ModelTopology`` eagerly; ``detect_topology``,
 ``TieredKVCache`` and ``KIVMiddleware`` on first access (they import
-transformers).
+transformers).  Beside it, with no counterpart in the reference: the paged
+cache of ragged batches (``PagedKVCache``, ``PagedBatch``, ``paged_append``)
+and ``norm_rope`` with its parameters.
 """
 
 __version__ = "0.1.0"
@@ -11,6 +13,8 @@ __version__ = "0.1.0"
 from .config import KIVConfig
 from .cold_store import ColdKVStore
 from .model_topology import ModelTopology
+from .paged import PagedBatch, PagedKVCache, paged_append
+from .rotary import HeadNorm, Rotary, norm_rope
 
 __all__ = [
     "KIVConfig",
@@ -19,6 +23,12 @@ __all__ = [
     "detect_topology",
     "TieredKVCache",
     "KIVMiddleware",
+    "HeadNorm",
+    "Rotary",
+    "norm_rope",
+    "PagedBatch",
+    "PagedKVCache",
+    "paged_append",
 ]
 
 _LAZY = {

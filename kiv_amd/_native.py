@@ -75,6 +75,56 @@ class AttentionArgs(C.Structure):
     ]
 
 
+_I64x2 = C.c_int64 * 2
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("inv_freq", C.c_void_p), ("axes", C.c_void_p), ("positions", C.c_void_p), ("position_stride", _I64x3),
+        ("position_bytes", C.c_int32), ("num_axes", C.c_int32), ("rot_dim", C.c_int32), ("interleaved", C.c_int32),
+        ("scale", C.c_float), ("_pad", C.c_int32),
+    ]
+
+
+class HeadNormArgs(C.Structure):
+    _fields_ = [("weight", C.c_void_p), ("eps", C.c_float), ("enabled", C.c_int32)]
+
+
+class NormRopeArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("tokens", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32), ("dtype", C.c_int32),
+        ("q", C.c_void_p), ("q_stride", _I64x3), ("q_out", C.c_void_p), ("q_out_stride", _I64x3),
+        ("k", C.c_void_p), ("k_stride", _I64x3), ("k_out", C.c_void_p), ("k_out_stride", _I64x3),
+        ("rotary", RotaryArgs), ("q_norm", HeadNormArgs), ("k_norm", HeadNormArgs),
+    ]
+
+
+class PagedCacheArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("stride", _I64x3), ("num_pages", C.c_int32), ("page_size", C.c_int32),
+        ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32), ("_pad", C.c_int32),
+    ]
+
+
+class PagedBatchArgs(C.Structure):
+    _fields_ = [
+        ("cu_q", C.c_void_p), ("kv_len", C.c_void_p), ("block_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("num_seqs", C.c_int32), ("table_width", C.c_int32), ("total_q", C.c_int32), ("max_q_len", C.c_int32),
+        ("max_kv_len", C.c_int32), ("_pad", C.c_int32),
+    ]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCacheArgs), ("batch", PagedBatchArgs),
+        ("k", C.c_void_p), ("k_stride", _I64x2), ("v", C.c_void_p), ("v_stride", _I64x2),
+        ("q", C.c_void_p), ("q_stride", _I64x2), ("q_out", C.c_void_p), ("q_out_stride", _I64x2),
+        ("num_q_heads", C.c_int32), ("_pad", C.c_int32),
+        ("rotary", RotaryArgs), ("q_norm", HeadNormArgs), ("k_norm", HeadNormArgs), ("v_norm", HeadNormArgs),
+    ]
+
+
 # Every symbol include/kiv_hip.h declares: name -> (restype, argtypes).
 SIGNATURES = {
     "kiv_version": (C.c_int, []),
@@ -101,6 +151,8 @@ SIGNATURES = {
     "kiv_retrieve_attend": (C.c_int, [C.c_void_p, C.POINTER(RetrieveArgs), C.POINTER(AttentionArgs), C.c_void_p]),
     "kiv_prefill_attention": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
     "kiv_prefill_workspace_size": (C.c_size_t, [C.c_int32] * 6),
+    "kiv_norm_rope": (C.c_int, [C.POINTER(NormRopeArgs), C.c_void_p]),
+    "kiv_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
 }
 
 _lock = threading.Lock()
@@ -166,6 +218,17 @@ def mask_kind(dtype: torch.dtype) -> int:
         raise TypeError(f"unsupported attention mask dtype {dtype}") from None
 
 
+def call(name: str, args: C.Structure, device: torch.device) -> None:
+    """Run entry point ``name`` on torch's current stream of ``device``, with
+    that device current."""
+    fn = getattr(lib(), name)
+    if device.index == torch.cuda.current_device():
+        check(fn(C.byref(args), stream_ptr(device)), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(C.byref(args), stream_ptr(device)), name)
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -183,7 +246,7 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-_ARRAYS = {3: _I64x3, 4: _I64x4}
+_ARRAYS = {2: _I64x2, 3: _I64x3, 4: _I64x4}
 _strides_cache: dict[tuple, C.Array] = {}
 
 

@@ -299,6 +299,30 @@ template <int DT> __device__ __forceinline__ f32x4_t mfma_16x16x32(const uint4 &
                                                    0, 0, 0);
 }
 
+// Two fp32 values rounded to the dtype (hardware conversion, nearest even),
+// packed low-first.
+template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == DT_BF16) return __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)a, (__bf16)b});
+  else return __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)a, (_Float16)b});
+}
+
+// The same on one 32x32 tile, K = 16.
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+template <int DT> __device__ __forceinline__ f32x16_t mfma_32x32x16(const uint4 &a, const uint4 &b, f32x16_t c) {
+  if constexpr (DT == DT_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                    c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                   0, 0, 0);
+}
+
+// Types of the LDS operands of loads straight into LDS and of transposing
+// LDS reads.
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+
 template <int DT> __device__ __forceinline__ float chunk_dot(const uint4 &x, const uint4 &q, float acc) {
   if constexpr (DT == DT_BF16) {
     acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x.x), __builtin_bit_cast(bf16x2_t, q.x), acc, false);

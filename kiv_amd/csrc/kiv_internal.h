@@ -45,6 +45,10 @@ struct DevBuf {
   void release();
 };
 
+// Argument checks of the paged cache's entry points (host only).
+int paged_cache_check(const kiv_paged_cache_t &c, const char *who);
+int paged_batch_check(const kiv_paged_batch_t &b, const kiv_paged_cache_t &c, const char *who);
+
 inline int elem_bytes(int dtype) { return dtype == KIV_DTYPE_F32 ? 4 : 2; }
 inline int vec_elems(int dtype) { return 16 / elem_bytes(dtype); }
 

@@ -120,13 +120,6 @@ __device__ __forceinline__ void float_bias4(const PrefillParams &p, int64_t o, f
     bias[i] = (p.mask_kind == KIV_MASK_F16 ? f16_bits_to_f32(w[i]) : bf16_bits_to_f32(w[i])) * kLog2e;
 }
 
-// Two fp32 values rounded to the dtype (hardware conversion, nearest even),
-// packed low-first.
-template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (DT == DT_BF16) return __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)a, (__bf16)b});
-  else return __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)a, (_Float16)b});
-}
-
 __device__ __forceinline__ int64_t mask_off(const PrefillParams &p, int b, int h, int i, int t) {
   return (int64_t)b * p.ms0 + (int64_t)h * p.ms1 + (int64_t)i * p.ms2 + (int64_t)t * p.ms3;
 }
@@ -665,19 +658,7 @@ __global__ void __launch_bounds__(kPfThreads) mask_tiles_kernel(PrefillParams p)
 //    same keys of dim l % 32, from two transposing LDS reads
 //    (ds_read_b64_tr_b16: each 16 lanes read 4 keys x 16 dims and lane n
 //    receives the 4 keys of dim n).
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-template <int DT> __device__ __forceinline__ f32x16_t mfma_32x32x16(const uint4 &a, const uint4 &b, f32x16_t c) {
-  if constexpr (DT == DT_BF16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
-                                                    c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
-                                                   0, 0, 0);
-}
 constexpr int kWaitMem = 0x0070;  // s_waitcnt vmcnt(0) lgkmcnt(0)
-typedef __attribute__((address_space(3))) void lds_void_t;
-typedef short i16x4_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 
 template <int DT, int KT, int MK> struct PfBlock32 : PfGeom<DT, KT, MK> {
   using Geom = PfGeom<DT, KT, MK>;

@@ -1,0 +1,180 @@
+"""Paged key/value cache: ragged batches of sequences of different lengths.
+
+The tiered cache grows one window for a whole batch; sequences that come, go
+and grow on their own are held here instead.  :class:`PagedKVCache` is one
+layer's pool of pages, :class:`PagedBatch` the new tokens of a step (packed
+one sequence behind the other, with each sequence's length and block table;
+built once a step and used for every layer), :func:`paged_append` writes the
+new keys and values to their pages with head norms and position rotation on
+the way, and :func:`paged_attention` attends over the pages: chunks of new
+tokens, single tokens, or both in one batch.
+
+Lengths and tables are read on the device only, so nothing here synchronises
+and a captured HIP graph follows what the arrays hold at each replay.  No
+counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native as nat
+from .rotary import HeadNorm, Rotary, aligned_rows, no_grad_check, out_rows
+
+
+class PagedKVCache:
+    """A pool of ``num_pages`` pages of ``page_size`` tokens of one layer's K and V.
+
+    ``k`` and ``v`` are [num_pages, num_kv_heads, page_size, head_dim] views;
+    with ``tokens_first`` a token's heads lie together in memory (head-major
+    pages otherwise).  The rows are uninitialised until appended.
+    """
+
+    def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+                 dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda",
+                 tokens_first: bool = False) -> None:
+        if min(num_pages, page_size, num_kv_heads, head_dim) < 1:
+            raise ValueError("num_pages, page_size, num_kv_heads and head_dim must be >= 1")
+        nat.dtype_code(dtype)
+        shape = ((num_pages, page_size, num_kv_heads, head_dim) if tokens_first
+                 else (num_pages, num_kv_heads, page_size, head_dim))
+        k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        self._bind(*(t.transpose(1, 2) if tokens_first else t for t in (k, v)))
+
+    @classmethod
+    def from_pages(cls, k: torch.Tensor, v: torch.Tensor) -> "PagedKVCache":
+        """A cache over existing [num_pages, num_kv_heads, page_size, head_dim]
+        tensors of equal shape, strides and dtype (any strides with unit
+        stride over head_dim)."""
+        self = cls.__new__(cls)
+        self._bind(k, v)
+        return self
+
+    def _bind(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("K and V pages must be equal [num_pages, num_kv_heads, page_size, head_dim] tensors")
+        if min(k.shape) < 1:
+            raise ValueError(f"empty pages {tuple(k.shape)}")
+        if k.stride() != v.stride():
+            raise ValueError("K and V pages must have the same strides")
+        if not k.is_cuda:
+            raise ValueError("the paged cache lives on a GPU")
+        out_rows(k, k, "K pages")
+        out_rows(v, v, "V pages")
+        self.k, self.v = k, v
+        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
+        self.dtype, self.device = k.dtype, k.device
+        self._args = nat.PagedCacheArgs(k.data_ptr(), v.data_ptr(), nat.strides(k, 3), self.num_pages, self.page_size,
+                                        self.num_kv_heads, self.head_dim, nat.dtype_code(k.dtype), 0)
+
+    def memory_bytes(self) -> int:
+        """Bytes of the pool's K and V rows."""
+        return 2 * self.k.numel() * self.k.element_size()
+
+
+class PagedBatch:
+    """The new tokens of one step, and the caches' sequences they belong to.
+
+    block_table  [S, W] int32: the pages of each sequence in order; entries
+                 outside the pool (-1, say) are pages that are not there.
+    kv_len       [S] int32: keys of each sequence, the new tokens' among them.
+    cu_q         [S + 1] int32: first packed row of each sequence and the end
+                 of the last; rows past it are no sequence's.  None: one new
+                 token a sequence.
+    max_q_len, max_kv_len  bounds of the lengths, known to the host; they
+                 choose the kernel only (a wrong one costs time, not results).
+                 Defaults: no bound.
+
+    The arrays stay the caller's: update them in place between steps (or
+    between replays of a captured graph).
+    """
+
+    def __init__(self, block_table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor | None = None,
+                 max_q_len: int | None = None, max_kv_len: int | None = None) -> None:
+        if block_table.dim() != 2 or kv_len.dim() != 1:
+            raise ValueError("block_table must be [S, W] and kv_len [S]")
+        for name, n in (("max_q_len", max_q_len), ("max_kv_len", max_kv_len)):
+            if n is not None and n < 0:
+                raise ValueError(f"{name} must not be negative, got {n}")
+        S, W = block_table.shape
+        if cu_q is None:
+            cu_q = torch.arange(S + 1, dtype=torch.int32, device=block_table.device)
+            max_q_len = 1
+        if kv_len.shape[0] != S or cu_q.dim() != 1 or cu_q.shape[0] != S + 1:
+            raise ValueError(f"block_table has {S} sequences, kv_len {tuple(kv_len.shape)}, cu_q {tuple(cu_q.shape)}")
+        for name, t in (("block_table", block_table), ("kv_len", kv_len), ("cu_q", cu_q)):
+            if t.dtype != torch.int32:
+                raise TypeError(f"{name} must be int32, not {t.dtype}")
+            if not t.is_cuda or t.device != block_table.device:
+                raise ValueError(f"{name} must be on the batch's GPU")
+            if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+                raise ValueError(f"{name} must have unit stride")
+        self.block_table, self.kv_len, self.cu_q = block_table, kv_len, cu_q
+        self.num_seqs, self.device = S, block_table.device
+        big = 2**31 - 1
+        self._args = nat.PagedBatchArgs(
+            cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0) if S > 1 else 0, S, W, 0,
+            big if max_q_len is None else min(max_q_len, big), big if max_kv_len is None else min(max_kv_len, big), 0)
+
+
+def _packed(t: torch.Tensor, name: str, cache: PagedKVCache, batch: PagedBatch, heads: int | None) -> torch.Tensor:
+    if t.dim() != 3 or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {cache.head_dim}], got {tuple(t.shape)}")
+    if t.dtype != cache.dtype:
+        raise TypeError(f"{name} is {t.dtype}, the cache {cache.dtype}")
+    if t.device != cache.device or batch.device != cache.device:
+        raise ValueError(f"{name} is on {t.device}, the batch on {batch.device}, the cache on {cache.device}")
+    return aligned_rows(t)
+
+
+def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor,
+                 q: torch.Tensor | None = None, positions: torch.Tensor | None = None, rotary: Rotary | None = None,
+                 q_norm: HeadNorm | None = None, k_norm: HeadNorm | None = None, v_norm: HeadNorm | None = None,
+                 q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Write the batch's new K and V rows [tokens, Hkv, D] to their pages.
+
+    Token r of sequence b goes to key index kv_len[b] - cu_q[b + 1] + r
+    (kv_len counts the new tokens), K normed (``k_norm``) and turned
+    (``rotary``) on the way, V normed (``v_norm``) or copied.  positions:
+    [tokens] or, with ``rotary.axes``, [axes, tokens]; None turns each token
+    by its key index.  With q [tokens, Hq, D] the queries are normed
+    (``q_norm``) and turned in the same launch, into ``q_out`` (new by
+    default; may be q); returns it, else None.  Rows past the last sequence
+    are left alone, in the pages and in ``q_out``; a token whose page is not
+    there is dropped.
+    """
+    no_grad_check("paged_append", q, k, v)
+    k = _packed(k, "k", cache, batch, cache.num_kv_heads)
+    v = _packed(v, "v", cache, batch, cache.num_kv_heads)
+    T = k.shape[0]
+    if v.shape[0] != T:
+        raise ValueError(f"k has {T} tokens, v {v.shape[0]}")
+    dev, D = cache.device, cache.head_dim
+    args = nat.PagedAppendArgs()
+    args.cache, args.batch = cache._args, batch._args
+    args.batch.total_q = T
+    args.k, args.k_stride = k.data_ptr(), nat.strides(k, 2)
+    args.v, args.v_stride = v.data_ptr(), nat.strides(v, 2)
+    if q is not None:
+        src = _packed(q, "q", cache, batch, None)
+        if src.shape[0] != T:
+            raise ValueError(f"k has {T} tokens, q {src.shape[0]}")
+        q_out = torch.empty_like(src) if q_out is None else out_rows(q_out, q, "q_out")
+        args.num_q_heads = q.shape[1]
+        args.q, args.q_stride = src.data_ptr(), nat.strides(src, 2)
+        args.q_out, args.q_out_stride = q_out.data_ptr(), nat.strides(q_out, 2)
+        if q_norm is not None:
+            args.q_norm = q_norm.check(D, dev)
+    elif q_norm is not None or q_out is not None:
+        raise ValueError("q_norm and q_out need q")
+    if k_norm is not None:
+        args.k_norm = k_norm.check(D, dev)
+    if v_norm is not None:
+        args.v_norm = v_norm.check(D, dev)
+    if rotary is not None:
+        args.rotary = rotary._args
+        rotary.fill(args.rotary, positions, 1, T, dev, batched=False)
+    elif positions is not None:
+        raise ValueError("positions need a rotation")
+    nat.call("kiv_paged_append", args, dev)
+    return q_out
