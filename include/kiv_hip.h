@@ -427,6 +427,34 @@ typedef struct {
  * one of their sequences. */
 int kiv_paged_append(const kiv_paged_append_args_t *args, kiv_stream_t stream);
 
+typedef struct {
+  kiv_paged_cache_t cache; /* head_dim 32, 64, 96, 128, 192 or 256 */
+  kiv_paged_batch_t batch;
+  const void *q;           /* [total_q, Hq, D], strides t, h */
+  int64_t q_stride[2];
+  void *out;               /* [total_q, Hq, D] contiguous */
+  int32_t num_q_heads;     /* Hq % Hkv == 0, q head h reads kv head h / (Hq / Hkv) */
+  int32_t window;          /* > 0: a token sees its own key and the window - 1 before it */
+  float scaling;           /* positive */
+  int32_t _pad;
+  void *workspace;         /* 256-byte aligned device scratch, fully rewritten by every call */
+  size_t workspace_bytes;
+} kiv_paged_attention_args_t;
+
+/* Workspace bytes kiv_paged_attention needs for these arguments, with the
+ * current device (0: refused arguments, or nothing to do). */
+size_t kiv_paged_attention_workspace_size(const kiv_paged_attention_args_t *args);
+
+/* One softmax per packed row and head over the keys of its sequence up to its
+ * own (the causal rule), in fp32; with fp16 and bf16 the probabilities are
+ * rounded to the dtype before they weight V.  Rows that see no key are zero;
+ * rows behind the last sequence are left as they are.  Values of keys that
+ * any row of the call sees must be finite: as in a product of matrices, a NaN
+ * in V reaches neighbouring rows whose weight for it is zero.  Rows past a
+ * sequence's length, and of other sequences, are never read.  Two calls may
+ * run at once if they have workspaces of their own. */
+int kiv_paged_attention(const kiv_paged_attention_args_t *args, kiv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

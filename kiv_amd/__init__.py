@@ -4,8 +4,8 @@ Same import surface as the reference package ``kiv`` (kiv/__init__.py:5-35):
 ``KIVConfig``, ``ColdKVStore`` and ``ModelTopology`` eagerly; ``detect_topology``,
 ``TieredKVCache`` and ``KIVMiddleware`` on first access (they import
 transformers).  Beside it, with no counterpart in the reference: the paged
-cache of ragged batches (``PagedKVCache``, ``PagedBatch``, ``paged_append``)
-and ``norm_rope`` with its parameters.
+cache of ragged batches (``PagedKVCache``, ``PagedBatch``, ``paged_append``,
+``paged_attention``) and ``norm_rope`` with its parameters.
 """
 
 __version__ = "0.1.0"
@@ -13,7 +13,7 @@ __version__ = "0.1.0"
 from .config import KIVConfig
 from .cold_store import ColdKVStore
 from .model_topology import ModelTopology
-from .paged import PagedBatch, PagedKVCache, paged_append
+from .paged import PagedBatch, PagedKVCache, paged_append, paged_attention
 from .rotary import HeadNorm, Rotary, norm_rope
 
 __all__ = [
@@ -29,6 +29,7 @@ __all__ = [
     "PagedBatch",
     "PagedKVCache",
     "paged_append",
+    "paged_attention",
 ]
 
 _LAZY = {

@@ -125,6 +125,14 @@ class PagedAppendArgs(C.Structure):
     ]
 
 
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCacheArgs), ("batch", PagedBatchArgs), ("q", C.c_void_p), ("q_stride", _I64x2),
+        ("out", C.c_void_p), ("num_q_heads", C.c_int32), ("window", C.c_int32), ("scaling", C.c_float),
+        ("_pad", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 # Every symbol include/kiv_hip.h declares: name -> (restype, argtypes).
 SIGNATURES = {
     "kiv_version": (C.c_int, []),
@@ -153,6 +161,8 @@ SIGNATURES = {
     "kiv_prefill_workspace_size": (C.c_size_t, [C.c_int32] * 6),
     "kiv_norm_rope": (C.c_int, [C.POINTER(NormRopeArgs), C.c_void_p]),
     "kiv_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "kiv_paged_attention": (C.c_int, [C.POINTER(PagedAttentionArgs), C.c_void_p]),
+    "kiv_paged_attention_workspace_size": (C.c_size_t, [C.POINTER(PagedAttentionArgs)]),
 }
 
 _lock = threading.Lock()

@@ -22,7 +22,7 @@ CSRC = PKG / "csrc"
 LIBDIR = PKG / "_lib"
 LIB = LIBDIR / "libkiv_hip.so"
 SOURCES = ("kiv_store.hip", "kiv_retrieve.hip", "kiv_attention.hip", "kiv_prefill.hip", "kiv_rotary.hip",
-           "kiv_probe.hip")
+           "kiv_paged.hip", "kiv_probe.hip")
 # Per-source flags.  The prefill attention keeps its MFMA accumulators in
 # ordinary VGPRs (the softmax rescales them every few tiles; in AGPRs every
 # tile would pay a copy in and out).

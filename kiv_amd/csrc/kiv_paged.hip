@@ -1,0 +1,720 @@
+// Attention of a ragged batch of new tokens over a paged K/V cache.
+//
+//   o_r = sum_j p_rj v_j,  p_rj = exp(s_rj - m_r) / sum_j exp(s_rj - m_r),
+//   s_rj = scaling * q_r . k_j over the keys j that row r sees (the causal
+//   rule, a sliding window, pages that are there), m_r their maximum.
+//
+// One pass over the keys with a running maximum and sum (base 2, fp32); the
+// query heads of one kv head are rows of one unit (kiv_paged_plan.h), so each
+// K and V row is read once for all of them.  The work of a call, in tiles of
+// keys, is dealt to the blocks in equal shares: a block finds its share from
+// the sequences' lengths itself (no launch, no host copy), takes its units
+// one after the other, and a unit that a share's end cuts is merged from
+// partial rows by paged_combine_kernel.
+//
+// paged_rows_kernel (single tokens, few rows, fp32): units of 16 rows, tiles
+// of 128 keys.  Each of a block's four waves takes 32 keys of a tile on its
+// own: K rows straight into registers as matrix operands, V rows through
+// registers into the wave's own LDS (read back transposed), the next tile's
+// rows in flight under this tile's softmax, no barrier until a unit ends.
+//   S^T = K Q^T with 16x16 matrix instructions: lane l gives key l % 16 of a
+//   16-key sub-tile (A) and query row l % 16 (B), 16-byte chunks l / 16 + 4 st
+//   of both, and receives keys 4 (l / 16) + i of the sub-tile for row l % 16.
+//   O^T += V^T P^T: B is the lane's own probabilities, A the same keys of dim
+//   l % 16 from the LDS.
+// Bound: memory (each K and V byte is used by at most 16 rows).
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "kiv_common.h"
+#include "kiv_internal.h"
+#include "kiv_paged_plan.h"
+
+namespace kiv {
+
+constexpr int kPgThreads = 256;
+constexpr int kPgWaves = kPgThreads / 64;
+constexpr float kPgLog2e = 1.4426950408889634f;
+constexpr float kPgSlack = 8.f;   // base-2 headroom before the running max moves
+constexpr int kRowsTileShift = 7;  // the rows kernel's tile: 128 keys
+constexpr int kRowsOfUnit = 16;
+
+// What the combine needs of a unit that block i continues: written by every
+// block (last < 0: nothing to merge here).
+struct PagedCut {
+  int row0, tokens, head0, heads;  // first packed row, tokens, first query head, heads (rows: tokens x heads)
+  int last;                        // the last block that has a part of it
+  int pad[3];
+};
+
+struct PagedAttnParams {
+  const char *q;
+  int64_t q_t, q_h;  // byte strides
+  const char *k, *v;
+  int64_t page_b, head_b, tok_b;  // byte strides of the pool
+  const int32_t *cu, *kv_len, *table;
+  int64_t table_stride;
+  int seqs, num_pages, page_size, hq;
+  FastDiv page_div;
+  PagedShape sh;
+  int blocks, least;  // most blocks that share the work, least tiles of a share
+  float scale_log2;
+  char *out;
+  PagedCut *cuts;  // [blocks]
+  float *ws_m, *ws_l, *ws_o;  // [2 blocks][rows], [2 blocks][rows][D]
+};
+
+// A row of zeros that stands for keys that are not there.
+__device__ const uint4 paged_zero_row[64] = {};
+
+// Tiles of a sequence's units of one kv head, by the whole wave (each lane
+// its own sequence; long ones by all lanes together).
+__device__ __forceinline__ int64_t paged_seq_weight(const PagedShape &sh, const PagedSeq &s) {
+  const int nrt = sh.row_tiles(s);
+  if (sh.whole) return nrt;
+  constexpr int kSerial = 4;
+  int64_t w = 0;
+  if (nrt <= kSerial)
+    for (int rt = 0; rt < nrt; ++rt) w += sh.weight(s, rt);
+  const int lane = threadIdx.x & 63;
+  for (uint64_t m = __ballot(nrt > kSerial); m; m &= m - 1) {
+    const int l = __builtin_ctzll(m), n = __shfl(nrt, l, 64);
+    const PagedSeq o{0, __shfl(s.qlen, l, 64), __shfl(s.len, l, 64)};
+    int64_t sum = 0;
+    for (int rt = lane; rt < n; rt += 64) sum += sh.weight(o, rt);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    if (lane == l) w = sum;
+  }
+  return w;
+}
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams &p, int b) {
+  return b < p.seqs ? p.sh.seq(p.cu[b], p.cu[b + 1], p.kv_len[b]) : PagedSeq{0, 0, 0};
+}
+__device__ __forceinline__ int64_t uniform_i64(int64_t x) { return (int64_t)uniform_u64((uint64_t)x); }
+
+// A block's place in the work: the unit it is at and what is left of its share.
+struct PagedWork {
+  int id;           // which share
+  int b, kvh, rt;   // the unit
+  PagedSeq s;
+  int nrt;
+  int64_t w, w_end, us;  // the share's next weight and end; the unit's first weight
+  PagedShares shares;
+
+  // Called by the whole block; false: there is no share for it.
+  __device__ __forceinline__ bool first(const PagedAttnParams &p) {
+    __shared__ int64_t sums[kPgWaves];
+    __shared__ int64_t found[3];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const PagedShape &sh = p.sh;
+    // All weights: thread tid's sequence of each kPgThreads, and the block's
+    // sums of them.
+    int64_t mine = 0, total = 0, incl = 0;
+    for (int base = 0; base < p.seqs; base += kPgThreads) {
+      mine = sh.hkv * paged_seq_weight(sh, paged_seq(p, base + tid));
+      total += scan(mine, incl, sums, wave, lane);
+    }
+    shares.total = total;
+    if (total == 0) return false;
+    shares.n = PagedShares::blocks(total, p.blocks, p.least);
+    if ((int)blockIdx.x >= shares.n) return false;
+    // Blocks are dealt to the eight dies in turn: a die takes neighbouring
+    // shares, which read the same keys through its L2.
+    id = !(shares.n & 7) ? ((int)blockIdx.x & 7) * (shares.n >> 3) + ((int)blockIdx.x >> 3) : (int)blockIdx.x;
+    w = shares.start(id);
+    w_end = shares.start(id + 1);
+    // The sequence that weight w falls in.
+    int64_t before = 0;
+    for (int base = 0; base < p.seqs; base += kPgThreads) {
+      int64_t sum = total;
+      if (p.seqs > kPgThreads) {
+        mine = sh.hkv * paged_seq_weight(sh, paged_seq(p, base + tid));
+        sum = scan(mine, incl, sums, wave, lane);
+      }
+      const int64_t end = before + incl;
+      if (w < end && w >= end - mine) {
+        found[0] = base + tid;
+        found[1] = end - mine;
+        found[2] = mine;
+      }
+      before += sum;
+      if (w < before) break;
+    }
+    __syncthreads();
+    b = (int)uniform_i64(found[0]);
+    const int64_t in = w - uniform_i64(found[1]), per_head = uniform_i64(found[2]) / sh.hkv;
+    s = paged_seq(p, b);
+    nrt = sh.row_tiles(s);
+    kvh = (int)(in / per_head);
+    int64_t r = in - kvh * per_head;  // weights of the head's units before w
+    if (sh.whole) {
+      rt = (int)r;
+      us = w;
+      return true;
+    }
+    for (rt = 0;; rt += 64) {
+      int64_t up = rt + lane < nrt ? sh.weight(s, rt + lane) : 0;
+      const int64_t n = up;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int64_t t = __shfl_up(up, d, 64);
+        if (lane >= d) up += t;
+      }
+      const uint64_t past = __ballot(up > r);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        rt += l;
+        us = w - (r - (__shfl(up, l, 64) - __shfl(n, l, 64)));
+        break;
+      }
+      r -= __shfl(up, 63, 64);
+    }
+    rt = (int)uniform_u32((uint32_t)rt);
+    us = uniform_i64(us);
+    return true;
+  }
+  // Inclusive sums over the block's threads; returns the block's.
+  static __device__ __forceinline__ int64_t scan(int64_t x, int64_t &incl, int64_t *sums, int wave, int lane) {
+    incl = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t t = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += t;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int i = 0; i < kPgWaves; ++i) {
+      const int64_t t = sums[i];
+      if (i < wave) incl += t;
+      all += t;
+    }
+    return uniform_i64(all);
+  }
+  // The unit behind this one; called while w < w_end.
+  __device__ __forceinline__ void next(const PagedAttnParams &p) {
+    us = w;
+    if (++rt < nrt) return;
+    rt = 0;
+    if (++kvh < p.sh.hkv) return;
+    kvh = 0;
+    do {
+      ++b;
+      s = paged_seq(p, b);
+      s.q0 = (int)uniform_u32(s.q0);
+      s.qlen = (int)uniform_u32(s.qlen);
+      s.len = (int)uniform_u32(s.len);
+      nrt = p.sh.row_tiles(s);
+    } while (nrt == 0 && b < p.seqs);
+  }
+};
+
+// One unit's rows and keys.
+struct PagedUnit {
+  int row0, tokens, head0, heads;  // first packed row, tokens, first query head, heads
+  int gw;
+  int64_t last0;   // last key that the first token sees
+  int k0, k1;      // keys that some row sees
+  __device__ __forceinline__ PagedUnit(const PagedShape &sh, const PagedSeq &s, int kvh, int rt) {
+    const int tok0 = sh.token0(rt), hg = sh.hpt == 1 ? 0 : rt % sh.hpt;
+    row0 = s.q0 + tok0;
+    tokens = sh.tokens(s, tok0);
+    head0 = kvh * sh.G + hg * sh.rows;
+    heads = min(sh.gw, sh.G - hg * sh.rows);
+    gw = sh.gw;
+    last0 = (int64_t)s.len - s.qlen + tok0;
+    sh.keys(s, rt, k0, k1);
+  }
+  // Packed row and query head of row r; false: the unit has no such row.
+  __device__ __forceinline__ bool row(int r, int &t, int &h) const {
+    const int tok = r / gw, g = r - tok * gw;
+    t = row0 + tok;
+    h = head0 + g;
+    return tok < tokens && g < heads;
+  }
+};
+
+// This block's part of a unit is [t0, t1) of its tiles: whole, or partial
+// rows in slot `partial`: 2 i of block i's first fragment where the unit
+// began before it, 2 i + 1 of the unit that goes on behind it.
+struct PagedPart {
+  int t0, t1, partial;
+  __device__ __forceinline__ PagedPart(const PagedAttnParams &p, PagedWork &wk, const PagedUnit &u) {
+    const int first = p.sh.first_tile(u.k0), n = p.sh.tiles(u.k0, u.k1);
+    if (p.sh.whole) {
+      t0 = first;
+      t1 = first + n;
+      partial = -1;
+      ++wk.w;
+      return;
+    }
+    const int64_t ue = wk.us + n, end = wk.w_end < ue ? wk.w_end : ue;
+    t0 = first + (int)(wk.w - wk.us);
+    t1 = first + (int)(end - wk.us);
+    const bool begins = wk.w == wk.us, ends = end == ue;
+    partial = begins && ends ? -1 : begins ? 2 * wk.id + 1 : 2 * wk.id;
+    wk.w = end;
+  }
+};
+
+// The cut in front of block id's share, if the block before it began the unit.
+__device__ __forceinline__ void paged_write_cut(const PagedAttnParams &p, const PagedWork &wk, const PagedUnit &u) {
+  if (!p.cuts || threadIdx.x != 0) return;
+  PagedCut c = {u.row0, u.tokens, u.head0, u.heads, -1, {0, 0, 0}};
+  if (!p.sh.whole && wk.w > wk.us && wk.us >= wk.shares.start(wk.id - 1))
+    c.last = wk.shares.block_of(wk.us + p.sh.tiles(u.k0, u.k1) - 1);
+  p.cuts[wk.id] = c;
+}
+__device__ __forceinline__ void paged_no_cut(const PagedAttnParams &p, int id) {
+  if (p.cuts && threadIdx.x == 0) p.cuts[id].last = -1;
+}
+
+template <int DT> __device__ __forceinline__ void store4(char *out, int64_t elem, const f32x4_t &o) {
+  if constexpr (DT == DT_F32) *reinterpret_cast<f32x4_t *>(out + 4 * elem) = o;
+  else *reinterpret_cast<uint2 *>(out + 2 * elem) = make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
+}
+
+// ---------------------------------------------------------------------------
+// Units of 16 rows.
+template <int DT, int D> struct RowsGeom {
+  static constexpr int EB = Elem<DT>::BYTES, RB = D * EB;  // bytes of a row
+  static constexpr int ST = RB / 64;                       // 64-byte steps of a row
+  static constexpr int VS = RB + 32;                       // LDS row stride: neighbouring keys 8 banks apart
+  static constexpr int ND = D / 16;
+  static constexpr int WAVE = 32 * VS;                     // LDS bytes of a wave: 32 V rows, later its 16 x D sums
+  static_assert(16 * D * 4 <= WAVE, "a wave's sums fit its V rows");
+};
+
+// acc += A B over one 64-byte step.
+template <int DT> __device__ __forceinline__ f32x4_t step_16x16(const uint4 &a, const uint4 &b, f32x4_t c) {
+  if constexpr (DT == DT_F32) {
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+  } else {
+    return mfma_16x16x32<DT>(a, b, c);
+  }
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kPgThreads) __attribute__((amdgpu_waves_per_eu(1, 4)))
+paged_rows_kernel(PagedAttnParams p) {
+  using Geo = RowsGeom<DT, D>;
+  constexpr int ST = Geo::ST, VS = Geo::VS, ND = Geo::ND;
+  __shared__ __align__(16) char vs[kPgWaves][Geo::WAVE];
+  __shared__ float wm[kPgWaves][16], wl[kPgWaves][16];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int col = lane & 15, grp = lane >> 4;
+  char *lds = vs[wave];
+  PagedWork wk;
+  if (!wk.first(p)) {
+    paged_no_cut(p, blockIdx.x);
+    return;
+  }
+  bool head = true;
+  while (wk.w < wk.w_end) {
+    const PagedUnit u(p.sh, wk.s, wk.kvh, wk.rt);
+    if (head) paged_write_cut(p, wk, u);
+    head = false;
+    const PagedPart part(p, wk, u);
+    // The lane's query row (rows the unit has not repeat its first).
+    int qt, qh;
+    const bool own = u.row(col, qt, qh);
+    const char *qp = p.q + (own ? qt : u.row0) * p.q_t + (own ? qh : u.head0) * p.q_h + 16 * grp;
+    uint4 qx[ST];
+#pragma unroll
+    for (int st = 0; st < ST; ++st) qx[st] = load16(qp + 64 * st);
+    const int64_t last = u.last0 + (own ? qt - u.row0 : 0), from = p.sh.window > 0 ? last - p.sh.window : -1;
+    const int32_t *table = p.table + wk.b * p.table_stride;
+    const char *kb = p.k + wk.kvh * p.head_b, *vb = p.v + wk.kvh * p.head_b;
+
+    f32x4_t o[ND];
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) o[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_lane = 0.f;
+
+    // The wave's 32 keys of tile t; the lane's are key0 + col and key0 + 16 +
+    // col: their pages' numbers (loaded two tiles ahead), then their rows.
+    auto key_of = [&](int t, int sub) { return (t << kRowsTileShift) + 32 * wave + 16 * sub + col; };
+    auto lookup = [&](int t, int (&page)[2]) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const int key = key_of(t, sub);
+        page[sub] = t < part.t1 && key >= u.k0 && key < u.k1 ? table[p.page_div.div(key)] : -1;
+      }
+    };
+    const char *kp[2], *vp[2];
+    uint32_t there = 0;  // of the tile in flight: bit 16 sub + k: its key k of sub-tile sub is there
+    auto resolve = [&](int t, const int (&page)[2]) {
+      there = 0;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const int key = key_of(t, sub);
+        const bool in = page[sub] >= 0 && page[sub] < p.num_pages;
+        const int slot = key - p.page_div.div(key) * p.page_size;
+        const int64_t off = page[sub] * p.page_b + slot * p.tok_b + 16 * grp;
+        const char *zero = reinterpret_cast<const char *>(paged_zero_row) + 16 * grp;
+        kp[sub] = in ? kb + off : zero;
+        vp[sub] = in ? vb + off : zero;
+        there |= (uint32_t)(__ballot(in) & 0xffffu) << (16 * sub);
+      }
+    };
+    uint4 kx[2][ST], vx[2][ST];
+    auto load_k = [&] {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int st = 0; st < ST; ++st) kx[sub][st] = load16(kp[sub] + 64 * st);
+    };
+    auto load_v = [&] {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int st = 0; st < ST; ++st) vx[sub][st] = load16(vp[sub] + 64 * st);
+    };
+    int page[2];
+    lookup(part.t0, page);
+    resolve(part.t0, page);
+    lookup(part.t0 + 1, page);
+    load_k();
+    load_v();
+    for (int t = part.t0; t < part.t1; ++t) {
+      const uint32_t seen = there;
+      f32x4_t s[2];
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        s[sub] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < ST; ++st) s[sub] = step_16x16<DT>(kx[sub][st], qx[st], s[sub]);
+      }
+      const bool more = t + 1 < part.t1;
+      if (more) {
+        resolve(t + 1, page);
+        lookup(t + 2, page);
+        load_k();
+      }
+      // V rows to LDS (this wave's alone; its reads of the tile before come
+      // first in the LDS queue).
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int st = 0; st < ST; ++st)
+          *reinterpret_cast<uint4 *>(lds + (16 * sub + col) * VS + 64 * st + 16 * grp) = vx[sub][st];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (more) load_v();
+
+      // Scores in base 2; keys that the row does not see are -inf.
+      const int key0 = key_of(t, 0) - col;
+      const bool edge = u.tokens > 1 && (key0 + 31 > u.last0 ||
+                                         (p.sh.window > 0 && key0 <= u.last0 + u.tokens - 1 - p.sh.window));
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[sub][i] *= p.scale_log2;
+      if (edge || seen != ~0u) {
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = 16 * sub + 4 * grp + i, key = key0 + at;
+            if (!((seen >> at) & 1u) || key > last || key <= from) s[sub][i] = -INFINITY;
+          }
+      }
+      // The running max moves only when a score exceeds it by 2^kPgSlack.
+      float x = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 4; ++i) x = fmaxf(x, s[0][i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x = fmaxf(x, s[1][i]);
+      if (__ballot(x > m_run + kPgSlack)) {
+        const float mt = half_wave_max(row_pair_max(x));
+        const float m_new = mt > m_run + kPgSlack ? mt : m_run;
+        const float a = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        l_lane *= a;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) o[dt] *= a;
+        m_run = m_new;
+      }
+      const float m_neg = m_run == -INFINITY ? 0.f : -m_run;
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] + m_neg);
+        l_lane += e[i];
+      }
+      if constexpr (DT == DT_F32) {
+        const char *at = lds + 4 * grp * VS + 4 * col;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float a = *reinterpret_cast<const float *>(at + (16 * (i >> 2) + (i & 3)) * VS + 64 * dt);
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, e[i], o[dt], 0, 0, 0);
+          }
+      } else {
+        // Probabilities are rounded to the dtype as matrix operands; their
+        // sum keeps the fp32 values.
+        const uint4 pb = make_uint4(pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]), pack2<DT>(e[4], e[5]),
+                                    pack2<DT>(e[6], e[7]));
+        const char *at = lds + (4 * grp + (col >> 2)) * VS + 8 * (col & 3);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          const uint2 lo =
+              __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t *)(at + 32 * dt)));
+          const uint2 hi = __builtin_bit_cast(
+              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t *)(at + 16 * VS + 32 * dt)));
+          o[dt] = mfma_16x16x32<DT>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb, o[dt]);
+        }
+      }
+    }
+
+    // The four waves' sums meet in LDS.
+    const float l_row = half_wave_sum(row_pair_sum(l_lane));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float *os = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) *reinterpret_cast<f32x4_t *>(os + col * D + 16 * dt + 4 * grp) = o[dt];
+    if (grp == 0) {
+      wm[wave][col] = m_run;
+      wl[wave][col] = l_row;
+    }
+    __syncthreads();
+    for (int i = tid; i < 16 * (D / 4); i += kPgThreads) {
+      const int r = i / (D / 4), d0 = 4 * (i - r * (D / 4));
+      int rt, rh;
+      if (!u.row(r, rt, rh)) continue;
+      float M = wm[0][r];
+#pragma unroll
+      for (int w = 1; w < kPgWaves; ++w) M = fmaxf(M, wm[w][r]);
+      float L = 0.f;
+      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kPgWaves; ++w) {
+        const float c = wm[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wm[w][r] - M);
+        L = fmaf(c, wl[w][r], L);
+        acc += c * *reinterpret_cast<const f32x4_t *>(reinterpret_cast<const float *>(vs[w]) + r * D + d0);
+      }
+      if (part.partial >= 0) {
+        const int64_t sr = (int64_t)part.partial * kRowsOfUnit + r;
+        *reinterpret_cast<f32x4_t *>(p.ws_o + sr * D + d0) = acc;
+        if (d0 == 0) {
+          p.ws_m[sr] = M;
+          p.ws_l[sr] = L;
+        }
+      } else {
+        // A row that sees no key gets zeros.
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+        store4<DT>(p.out, ((int64_t)rt * p.hq + rh) * D + d0, acc * inv);
+      }
+    }
+    __syncthreads();  // the next unit's V rows reuse the LDS
+    if (wk.w < wk.w_end) wk.next(p);
+  }
+}
+
+// Merges the units that the shares cut: o = sum_i 2^(m_i - M) o_i / sum_i
+// 2^(m_i - M) l_i over a unit's partial rows, M the largest of their maxima.
+// Grid (shares, rows / 4): one wave a row, its lanes D / 4 dims wide times the
+// parts side by side; blocks of shares that continue no unit leave at once.
+constexpr int kCombineParts = 4;  // parts of a lane in flight together
+template <int DT> __global__ void __launch_bounds__(kPgThreads) paged_combine_kernel(PagedAttnParams p, int D) {
+  const int id = blockIdx.x;
+  const PagedCut c = p.cuts[id];
+  if (c.last < 0) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r = blockIdx.y * kPgWaves + wave, gw = p.sh.gw, tok = r / gw, g = r - tok * gw;
+  if (r >= p.sh.rows || tok >= c.tokens || g >= c.heads) return;
+  const int n = c.last - id + 2;  // the part of the block before, then parts id .. last
+  const int wide = D / 4 <= 64 ? D / 4 : 64, side = 64 / wide, mine = lane / wide, d0 = 4 * (lane - mine * wide);
+  auto at = [&](int i) { return (int64_t)(i == 0 ? 2 * id - 1 : 2 * (id + i - 1)) * p.sh.rows + r; };
+  float M = -INFINITY, L = 0.f;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  if (mine < side) {
+    for (int i0 = mine; i0 < n; i0 += kCombineParts * side) {
+      float ms[kCombineParts], ls[kCombineParts];
+      f32x4_t os[kCombineParts];
+#pragma unroll
+      for (int k = 0; k < kCombineParts; ++k) {
+        const bool in = i0 + k * side < n;
+        const int64_t x = at(in ? i0 + k * side : i0);
+        ms[k] = in ? p.ws_m[x] : -INFINITY;
+        ls[k] = in ? p.ws_l[x] : 0.f;
+        os[k] = *reinterpret_cast<const f32x4_t *>(p.ws_o + x * D + d0);
+      }
+      float m = M;
+#pragma unroll
+      for (int k = 0; k < kCombineParts; ++k) m = fmaxf(m, ms[k]);
+      if (m == -INFINITY) continue;
+      const float a = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m);
+      L *= a;
+      acc *= a;
+#pragma unroll
+      for (int k = 0; k < kCombineParts; ++k) {
+        const float w = ms[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[k] - m);
+        L = fmaf(w, ls[k], L);
+        acc += w * os[k];
+      }
+      M = m;
+    }
+  }
+  // The sides' sums: lane mine * wide + d adds those of the other sides.
+  float MM = M;
+  for (int k = 1; k < side; ++k) MM = fmaxf(MM, __shfl(M, (lane + k * wide) % (side * wide), 64));
+  const float a = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - MM);
+  L *= a;
+  acc *= a;
+  float LL = L;
+  f32x4_t sum = acc;
+  for (int k = 1; k < side; ++k) {
+    const int from = (lane + k * wide) % (side * wide);
+    LL += __shfl(L, from, 64);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] += __shfl(acc[j], from, 64);
+  }
+  if (mine != 0) return;
+  const float inv = LL > 0.f ? 1.f / LL : 0.f;
+  store4<DT>(p.out, ((int64_t)(c.row0 + tok) * p.hq + c.head0 + g) * D + d0, sum * inv);
+}
+
+// ------------------------------------------------------------------- host
+struct PagedPlan {
+  PagedShape sh;
+  int blocks, least;
+  size_t m_off, l_off, o_off, total;  // workspace: cuts, then these
+};
+
+static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
+  const kiv_paged_cache_t &c = a.cache;
+  const kiv_paged_batch_t &b = a.batch;
+  PagedPlan w;
+  const int G = a.num_q_heads / c.num_kv_heads, cap = b.table_width * c.page_size;
+  const int64_t most_keys = std::min<int64_t>(b.max_kv_len, cap);
+  const int rows = kRowsOfUnit, shift = kRowsTileShift;
+  w.sh = PagedShape::of(b.total_q, c.num_kv_heads, G, rows, cap, shift, a.window, false);
+  // More than the call's units and tiles, by what the host knows of them.
+  const int64_t units =
+      ((int64_t)b.total_q / w.sh.tpu + std::min(b.num_seqs, b.total_q)) * w.sh.hpt * c.num_kv_heads;
+  const int64_t keys = a.window > 0 ? std::min<int64_t>(most_keys, (int64_t)a.window + w.sh.tpu) : most_keys;
+  const int64_t tiles = (keys >> shift) + 2;
+  w.least = 1;
+  w.blocks = (int)std::max<int64_t>(8, std::min<int64_t>(2 * device_cu_count(), units * tiles) & ~int64_t(7));
+  auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+  const size_t parts = (size_t)2 * w.blocks * rows;
+  w.m_off = up(w.blocks * sizeof(PagedCut));
+  w.l_off = w.m_off + up(parts * 4);
+  w.o_off = w.l_off + up(parts * 4);
+  w.total = w.o_off + parts * c.head_dim * 4;
+  return w;
+}
+
+static int paged_attention_check(const kiv_paged_attention_args_t *a, const char *who) {
+  if (!a) return fail(KIV_ERR_INVALID, "%s: null argument", who);
+  const kiv_paged_cache_t &c = a->cache;
+  int rc = paged_cache_check(c, who);
+  if (rc || (rc = paged_batch_check(a->batch, c, who))) return rc;
+  const int D = c.head_dim, kt = D / 32;
+  if (D % 32 || !(kt <= 4 || kt == 6 || kt == 8))
+    return fail(KIV_ERR_UNSUPPORTED, "%s: head_dim %d unsupported (32, 64, 96, 128, 192, 256)", who, D);
+  if (a->num_q_heads < 1 || a->num_q_heads % c.num_kv_heads)
+    return fail(KIV_ERR_INVALID, "%s: bad head geometry", who);
+  if (a->window < 0) return fail(KIV_ERR_INVALID, "%s: negative window", who);
+  // Hidden scores are -inf behind the scale, and the maximum is taken there.
+  if (!(a->scaling > 0.f) || !(a->scaling < INFINITY))
+    return fail(KIV_ERR_UNSUPPORTED, "%s: scaling must be positive and finite", who);
+  return KIV_OK;
+}
+
+template <typename F> static int with_head_dim(int D, F &&f) {
+  using std::integral_constant;
+  switch (D) {
+    case 32: return f(integral_constant<int, 32>{});
+    case 64: return f(integral_constant<int, 64>{});
+    case 96: return f(integral_constant<int, 96>{});
+    case 128: return f(integral_constant<int, 128>{});
+    case 192: return f(integral_constant<int, 192>{});
+    default: return f(integral_constant<int, 256>{});
+  }
+}
+
+}  // namespace kiv
+
+using namespace kiv;
+
+extern "C" {
+
+size_t kiv_paged_attention_workspace_size(const kiv_paged_attention_args_t *a) {
+  if (paged_attention_check(a, "kiv_paged_attention_workspace_size")) return 0;
+  if (a->batch.total_q == 0 || a->batch.num_seqs == 0) return 0;
+  return paged_plan(*a).total;
+}
+
+int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream) {
+  const char *who = "kiv_paged_attention";
+  int rc = paged_attention_check(a, who);
+  if (rc) return rc;
+  const kiv_paged_cache_t &c = a->cache;
+  const kiv_paged_batch_t &b = a->batch;
+  if (b.total_q == 0 || b.num_seqs == 0) return KIV_OK;
+  if (!a->q || !a->out) return fail(KIV_ERR_INVALID, "%s: null pointer", who);
+  const int eb = elem_bytes(c.dtype), vec = vec_elems(c.dtype);
+  if ((((uintptr_t)a->q | (uintptr_t)a->out) & 15) || a->q_stride[0] % vec || a->q_stride[1] % vec)
+    return fail(KIV_ERR_INVALID, "%s: rows must be 16-byte aligned", who);
+  const PagedPlan w = paged_plan(*a);
+  if (!a->workspace || a->workspace_bytes < w.total || ((uintptr_t)a->workspace & 255))
+    return fail(KIV_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes "
+                "(kiv_paged_attention_workspace_size)", who, w.total);
+  PagedAttnParams p;
+  p.q = (const char *)a->q;
+  p.q_t = a->q_stride[0] * eb;
+  p.q_h = a->q_stride[1] * eb;
+  p.k = (const char *)c.k;
+  p.v = (const char *)c.v;
+  p.page_b = c.stride[0] * eb;
+  p.head_b = c.stride[1] * eb;
+  p.tok_b = c.stride[2] * eb;
+  p.cu = b.cu_q;
+  p.kv_len = b.kv_len;
+  p.table = b.block_table;
+  p.table_stride = b.table_stride;
+  p.seqs = b.num_seqs;
+  p.num_pages = c.num_pages;
+  p.page_size = c.page_size;
+  p.hq = a->num_q_heads;
+  p.page_div = FastDiv::of(c.page_size);
+  p.sh = w.sh;
+  p.blocks = w.blocks;
+  p.least = w.least;
+  p.scale_log2 = a->scaling * kPgLog2e;
+  p.out = (char *)a->out;
+  char *ws = (char *)a->workspace;
+  p.cuts = (PagedCut *)ws;
+  p.ws_m = (float *)(ws + w.m_off);
+  p.ws_l = (float *)(ws + w.l_off);
+  p.ws_o = (float *)(ws + w.o_off);
+  hipStream_t st = (hipStream_t)stream;
+  const int D = c.head_dim;
+  return with_head_dim(D, [&](auto dc) {
+    constexpr int DV = decltype(dc)::value;
+    const dim3 grid((unsigned)p.blocks), cgrid((unsigned)p.blocks, (unsigned)((p.sh.rows + kPgWaves - 1) / kPgWaves));
+    auto go = [&](auto dtc) {
+      constexpr int DTV = decltype(dtc)::value;
+      hipLaunchKernelGGL((paged_rows_kernel<DTV, DV>), grid, dim3(kPgThreads), 0, st, p);
+      hipLaunchKernelGGL((paged_combine_kernel<DTV>), cgrid, dim3(kPgThreads), 0, st, p, D);
+    };
+    if (c.dtype == KIV_DTYPE_F32) go(std::integral_constant<int, DT_F32>{});
+    else if (c.dtype == KIV_DTYPE_F16) go(std::integral_constant<int, DT_F16>{});
+    else go(std::integral_constant<int, DT_BF16>{});
+    KIV_HIP(hipGetLastError());
+    return (int)KIV_OK;
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,115 @@
+// How the paged attention's work is cut into units and dealt to blocks.
+// Plain C++ beside the kernels that use it, so that the arithmetic is also
+// checked on the host.
+#pragma once
+
+#include <stdint.h>
+
+#if defined(__HIPCC__)
+#define KIV_HD __host__ __device__
+#else
+#define KIV_HD
+#endif
+
+namespace kiv {
+
+// Quotients of 31-bit numbers by a fixed divisor: n / d == (n * mul) >> shift.
+// With l = ceil(log2 d), mul = floor(2^(31 + l) / d) + 1 exceeds 2^(31 + l) / d
+// by less than 1 <= 2^l / d, so n * mul / 2^(31 + l) exceeds n / d by less
+// than n / 2^(31) / d < 1 / d.
+struct FastDiv {
+  uint32_t mul;
+  int shift;
+  static FastDiv of(int d) {
+    int l = 0;
+    while ((int64_t(1) << l) < d) ++l;
+    return FastDiv{(uint32_t)((uint64_t(1) << (31 + l)) / (uint64_t)d + 1), 31 + l};
+  }
+  KIV_HD int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+};
+
+// A sequence as the kernels take it: its packed rows [q0, q0 + qlen) and its
+// length, brought into range whatever the arrays hold.
+struct PagedSeq {
+  int q0, qlen, len;
+};
+
+// A unit is the query rows of one kv head that one block (or several, over
+// shares of its keys) attends together: tpu tokens times the G query heads of
+// the kv head, at most `rows` rows; with more heads than rows, one token and
+// one of hpt groups of heads.  Row r of a unit is its token r / gw, head
+// r % gw.  The units of a sequence are numbered kv heads first, then tokens
+// (neighbouring shares read the same keys), then head groups.
+struct PagedShape {
+  int total_q, hkv, G;
+  int rows, tpu, hpt, gw;
+  int cap;         // keys the block table spans
+  int tile_shift;  // keys of a tile: 1 << tile_shift
+  int window;      // 0: none
+  int whole;       // a unit is never divided (its weight is one)
+
+  static PagedShape of(int total_q, int hkv, int G, int rows, int cap, int tile_shift, int window, bool whole) {
+    PagedShape s;
+    s.total_q = total_q;
+    s.hkv = hkv;
+    s.G = G;
+    s.rows = rows;
+    s.tpu = G < rows ? rows / G : 1;
+    s.hpt = (G + rows - 1) / rows;
+    s.gw = G < rows ? G : rows;
+    s.cap = cap;
+    s.tile_shift = tile_shift;
+    s.window = window;
+    s.whole = whole;
+    return s;
+  }
+  KIV_HD PagedSeq seq(int cu0, int cu1, int len) const {
+    PagedSeq q;
+    q.q0 = cu0 < 0 ? 0 : cu0 > total_q ? total_q : cu0;
+    const int end = cu1 < 0 ? 0 : cu1 > total_q ? total_q : cu1;
+    q.qlen = end > q.q0 ? end - q.q0 : 0;
+    q.len = len < 0 ? 0 : len;
+    return q;
+  }
+  // Units of one kv head of a sequence.
+  KIV_HD int row_tiles(const PagedSeq &s) const { return (s.qlen + tpu - 1) / tpu * hpt; }
+  KIV_HD int token0(int rt) const { return (hpt == 1 ? rt : rt / hpt) * tpu; }
+  KIV_HD int tokens(const PagedSeq &s, int tok0) const { return s.qlen - tok0 < tpu ? s.qlen - tok0 : tpu; }
+  // Keys [k0, k1) that some row of unit rt sees.
+  KIV_HD void keys(const PagedSeq &s, int rt, int &k0, int &k1) const {
+    const int tok0 = token0(rt);
+    const int64_t off = (int64_t)s.len - s.qlen, last = off + tok0 + tokens(s, tok0);
+    const int64_t first = window > 0 ? off + tok0 - window + 1 : 0;
+    k1 = (int)(last < 0 ? 0 : last < cap ? last : cap);
+    k0 = (int)(first < 0 ? 0 : first < k1 ? first : k1);
+    if (k0 >= k1) k0 = k1 = 0;
+  }
+  // First tile and number of tiles of the keys [k0, k1); a unit that sees no
+  // key has one, so that a block writes its rows.
+  KIV_HD int first_tile(int k0) const { return k0 >> tile_shift; }
+  KIV_HD int tiles(int k0, int k1) const { return k0 < k1 ? ((k1 - 1) >> tile_shift) - (k0 >> tile_shift) + 1 : 1; }
+  KIV_HD int weight(const PagedSeq &s, int rt) const {
+    if (whole) return 1;
+    int k0, k1;
+    keys(s, rt, k0, k1);
+    return tiles(k0, k1);
+  }
+};
+
+// The weights 0 .. total - 1 in n shares, equal to within one: block i takes
+// [start(i), start(i + 1)).
+struct PagedShares {
+  int64_t total;
+  int n;
+  // Blocks that share the work: none gets less than `least`, a multiple of
+  // the eight dies where there are that many.
+  KIV_HD static int blocks(int64_t total, int most, int least) {
+    const int64_t n = total / least;
+    const int m = (int)(n < most ? n : most);
+    return m >= 8 ? m & ~7 : m > 0 ? m : 1;
+  }
+  KIV_HD int64_t start(int i) const { return total * i / n; }
+  KIV_HD int block_of(int64_t w) const { return (int)(((w + 1) * n - 1) / total); }
+};
+
+}  // namespace kiv

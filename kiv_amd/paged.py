@@ -178,3 +178,44 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
         raise ValueError("positions need a rotation")
     nat.call("kiv_paged_append", args, dev)
     return q_out
+
+
+def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, scaling: float, window: int = 0,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(q K^T * scaling) V of the batch's packed rows [tokens, Hq, D]
+    over the keys of their sequences, up to each token's own
+    (kv_len[b] - cu_q[b + 1] + row); with ``window`` the last ``window`` of
+    those.  Append the new tokens first.  Query head h reads key head
+    h // (Hq / Hkv); head_dim 32, 64, 96, 128, 192 or 256.
+
+    Returns [tokens, Hq, D]: ``out`` (contiguous) or a new tensor.  Rows that
+    see no key are zero; rows past the last sequence stay as they are (in a
+    new tensor: undefined).
+    """
+    no_grad_check("paged_attention", query)
+    q = _packed(query, "query", cache, batch, None)
+    T, hq, D = q.shape
+    if out is None:
+        out = torch.empty((T, hq, D), dtype=q.dtype, device=q.device)
+    elif out_rows(out, query, "out") is not None and not out.is_contiguous():
+        raise ValueError("out must be contiguous")
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    args = nat.PagedAttentionArgs()
+    args.cache, args.batch = cache._args, batch._args
+    args.batch.total_q = T
+    args.q, args.q_stride = q.data_ptr(), nat.strides(q, 2)
+    args.out = out.data_ptr()
+    args.num_q_heads, args.window, args.scaling = hq, min(window, 2**31 - 1), scaling
+    ws = _workspace(args, cache.device)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
+    nat.call("kiv_paged_attention", args, cache.device)
+    return out
+
+
+def _workspace(args: nat.PagedAttentionArgs, device: torch.device) -> torch.Tensor:
+    """Scratch of one call, from torch's allocator on the current stream: calls
+    on other streams, and captured graphs, have their own."""
+    with torch.cuda.device(device):
+        need = nat.lib().kiv_paged_attention_workspace_size(args)
+    return torch.empty(need, dtype=torch.uint8, device=device)

@@ -108,3 +108,20 @@ def make_table(lens, page, pages, g, width=None, extra=0):
         for j in range(n):
             t[b, j] = order.pop()
     return t
+
+
+def attention_bound(ref, mag, q, k_pages, dtype, scaling, n):
+    """The store's rounding; the probabilities' rounding to the dtype (16-bit
+    types; fp16 also loses those below its smallest number); and fp32 steps:
+    a score's D products and sums (relative to the largest sum of |q k|, S),
+    which moves a probability by as much and the normalised sum by twice
+    that, and n additions of the weighted sum with the exponentials' few."""
+    u, D = half_step(dtype), q.shape[-1]
+    S = float(q.double().abs().amax() * k_pages.double().abs().nan_to_num(0.0).amax()) * D * scaling
+    # |q|_2 |k|_2 bounds sum |q k| far closer where rows are long.
+    S = min(S, float(q.double().norm(dim=-1).amax() * k_pages.double().nan_to_num(0.0).norm(dim=-1).amax()) * scaling)
+    fp32 = (2 * (D + 8) * S + n + 64) * U32
+    bound = u * ref.abs() + (fp32 + (0.0 if dtype == torch.float32 else u)) * mag + 1e-30
+    if dtype == torch.float16:
+        bound = bound + n * 2.0 ** -25 * mag.amax() + 2.0 ** -25
+    return bound

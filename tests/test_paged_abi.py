@@ -21,6 +21,7 @@ STRUCTS = {
     "kiv_paged_cache_t": nat.PagedCacheArgs,
     "kiv_paged_batch_t": nat.PagedBatchArgs,
     "kiv_paged_append_args_t": nat.PagedAppendArgs,
+    "kiv_paged_attention_args_t": nat.PagedAttentionArgs,
 }
 AT = 1 << 20  # an aligned address that no refused call follows
 
@@ -137,6 +138,50 @@ def test_paged_append_refusals(code, over):
     lib = nat.lib()
     assert lib.kiv_paged_append(C.byref(append_args(**over)), None) == code
     assert b"kiv_paged_append" in lib.kiv_last_error()
+
+
+def attention_args(**over):
+    a = nat.PagedAttentionArgs()
+    fill_cache(a)
+    a.q = a.out = a.workspace = AT
+    a.q_stride = (C.c_int64 * 2)(256, 64)
+    a.num_q_heads, a.scaling, a.workspace_bytes = 4, 0.125, 1 << 40
+    for name, value in over.items():
+        obj, _, field = name.rpartition("__")
+        setattr(getattr(a, obj) if obj else a, field, value)
+    return a
+
+
+@pytest.mark.parametrize("code,over", CACHE_REFUSALS + [
+    (nat.ERR_INVALID, dict(q=None)),
+    (nat.ERR_INVALID, dict(out=AT + 8)),
+    (nat.ERR_INVALID, dict(q_stride=(C.c_int64 * 2)(256, 60))),
+    (nat.ERR_INVALID, dict(num_q_heads=3)),
+    (nat.ERR_INVALID, dict(num_q_heads=0)),
+    (nat.ERR_INVALID, dict(window=-1)),
+    (nat.ERR_UNSUPPORTED, dict(cache__head_dim=48)),
+    (nat.ERR_UNSUPPORTED, dict(cache__head_dim=512)),
+    (nat.ERR_UNSUPPORTED, dict(scaling=0.0)),
+    (nat.ERR_UNSUPPORTED, dict(scaling=float("nan"))),
+    (nat.ERR_UNSUPPORTED, dict(scaling=float("inf"))),
+    (nat.ERR_INVALID, dict(workspace=None)),
+    (nat.ERR_INVALID, dict(workspace=AT + 16)),
+    (nat.ERR_INVALID, dict(workspace_bytes=64)),
+])
+def test_paged_attention_refusals(code, over):
+    lib = nat.lib()
+    assert lib.kiv_paged_attention(C.byref(attention_args(**over)), None) == code
+    assert b"kiv_paged_attention" in lib.kiv_last_error()
+
+
+def test_paged_workspace_size():
+    lib = nat.lib()
+    assert lib.kiv_paged_attention_workspace_size(None) == 0
+    assert lib.kiv_paged_attention_workspace_size(C.byref(attention_args(cache__head_dim=48))) == 0
+    assert lib.kiv_paged_attention_workspace_size(C.byref(attention_args(batch__total_q=0))) == 0
+    assert lib.kiv_paged_attention_workspace_size(C.byref(attention_args())) > 0
+    assert lib.kiv_paged_attention(C.byref(attention_args(batch__total_q=0, workspace=None)), None) == 0
+    assert lib.kiv_paged_attention(None, None) == nat.ERR_INVALID
 
 
 def test_cpu_tensors_are_refused():
