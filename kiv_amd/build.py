@@ -26,7 +26,8 @@ SOURCES = ("kiv_store.hip", "kiv_retrieve.hip", "kiv_attention.hip", "kiv_prefil
 # Per-source flags.  The prefill attention keeps its MFMA accumulators in
 # ordinary VGPRs (the softmax rescales them every few tiles; in AGPRs every
 # tile would pay a copy in and out).
-EXTRA = {"kiv_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]}
+EXTRA = {"kiv_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+         "kiv_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]}
 ARCH = os.environ.get("KIV_OFFLOAD_ARCH", "gfx950")
 
 COMMON = [

@@ -520,6 +520,337 @@ paged_rows_kernel(PagedAttnParams p) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Units of many rows (16-bit types): 4 waves of RG groups of 32 rows.
+//
+// K and V tiles of 64 keys go from their pages straight to LDS, as rows,
+// double-buffered, their 16-byte chunks permuted so that operand reads spread
+// over the banks (K chunk c of row r at c ^ xk(r), V chunk c at c ^ 4 xv(r):
+// the loading lanes fetch the permuted chunk).  A wave reads each operand
+// once for its RG groups.
+//   S^T = K Q^T with 32x32 matrix instructions: lane l gives row l % 32 of a
+//   32-key sub-tile of K (A) and its own query row l % 32 (B, in registers
+//   for the whole unit), dims 16 st + 8 (l / 32) .. + 7 of step st, and
+//   receives keys 8 (i / 4) + 4 (l / 32) + i % 4 (i < 16) for its row.
+//   O^T += V^T P^T, 16 keys a step: B is the lane's own probabilities, A the
+//   same keys of dim l % 32 from two transposing LDS reads.
+// One iteration forms the scores of the next tile beside the exponentials of
+// this one, then adds this tile's values beside the next one's maxima, so
+// that vector and matrix instructions alternate in one wave's stream.
+template <int DT, int KT, int RG> struct ChunkGeom {
+  static constexpr int D = 32 * KT, CPR = D / 8;
+  static constexpr int CP = CPR <= 4 ? 4 : CPR <= 8 ? 8 : CPR <= 16 ? 16 : 32;  // chunks of an LDS row
+  static constexpr int RPI = 64 / CP;   // rows of a load instruction
+  static constexpr int NJ = CP / 4;     // load instructions of a wave for a tile of K (of V)
+  static constexpr int TILE = 64 * CP * 16;  // LDS bytes of a tile
+  static constexpr int KS = D / 16, ND = D / 32;
+  static constexpr int ROWS = 128 * RG;
+  static __device__ __forceinline__ int xk(int r) { return CP >= 16 ? r & 15 : (r / (16 / CP)) & (CP - 1); }
+  static __device__ __forceinline__ int xv(int r) { return CP >= 16 ? r & 3 : CP == 8 ? (r >> 1) & 1 : 0; }
+};
+constexpr int kChunkTileShift = 6;
+constexpr int kPgWaitAll = 0x0070;  // s_waitcnt vmcnt(0) lgkmcnt(0)
+typedef __attribute__((address_space(1))) const void gbl_void_t;
+
+__device__ __forceinline__ void lds_load16(const char *from, char *to) {
+  __builtin_amdgcn_global_load_lds((gbl_void_t *)from, (lds_void_t *)to, 16, 0, 0);
+}
+
+template <int DT, int KT, int RG>
+__global__ void __launch_bounds__(kPgThreads, 1) paged_chunk_kernel(PagedAttnParams p) {
+  using Geo = ChunkGeom<DT, KT, RG>;
+  constexpr int D = Geo::D, CP = Geo::CP, CPR = Geo::CPR, RPI = Geo::RPI, NJ = Geo::NJ, KS = Geo::KS, ND = Geo::ND;
+  // Objects of their own, so that the compiler knows that reads of one do not
+  // wait for loads into another.
+  __shared__ __align__(1024) char kb0[Geo::TILE], kb1[Geo::TILE], vb0[Geo::TILE], vb1[Geo::TILE];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int row = lane & 31, hf = lane >> 5;
+  PagedWork wk;
+  if (!wk.first(p)) {
+    paged_no_cut(p, blockIdx.x);
+    return;
+  }
+  // Loads: the lane's row of the wave's first instruction (the next ones are
+  // 4 RPI rows on) and its chunks' bytes; with 32 chunks the rows' K
+  // permutation alternates.
+  const int lrow = wave * RPI + lane / CP, pc = lane % CP;
+  const int kc0 = min(pc ^ Geo::xk(lrow), CPR - 1) * 16, kc1 = min(pc ^ Geo::xk(lrow + 4 * RPI), CPR - 1) * 16;
+  const int vc = min(pc ^ (4 * Geo::xv(lrow)), CPR - 1) * 16;
+  // Operand reads: the lane's byte offsets within a tile.
+  const int kaddr = row * CP * 16 + ((hf ^ Geo::xk(row)) << 4);
+  int vaddr[ND];
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt) {
+    const int j16 = lane & 15, q = j16 >> 2;  // the transposing read: key q of four, dims 4 (j16 % 4) ..
+    const int c = 4 * (dt ^ Geo::xv(q)) + 2 * ((lane >> 4) & 1) + ((j16 & 3) >> 1);
+    vaddr[dt] = (4 * hf + q) * CP * 16 + c * 16 + (j16 & 1) * 8;
+  }
+  const bool whole_groups = p.page_size % RPI == 0;  // a load instruction's rows lie in one page
+  const float cc = p.scale_log2;
+  bool head = true;
+  while (wk.w < wk.w_end) {
+    const PagedUnit u(p.sh, wk.s, wk.kvh, wk.rt);
+    if (head) paged_write_cut(p, wk, u);
+    head = false;
+    const PagedPart part(p, wk, u);
+    const int32_t *table = p.table + wk.b * p.table_stride;
+    const char *kbase = p.k + wk.kvh * p.head_b, *vbase = p.v + wk.kvh * p.head_b;
+
+    // Pages of tile t's keys, a key a lane (-1 past the table).
+    auto lookup = [&](int t) {
+      const int key = (t << kChunkTileShift) + lane;
+      return t < part.t1 && key < p.sh.cap ? table[p.page_div.div(key)] : -1;
+    };
+    // Which of them are there (and seen by some row of the unit).
+    auto present = [&](int t, int page) {
+      const int key = (t << kChunkTileShift) + lane;
+      return __ballot(page >= 0 && page < p.num_pages && key >= u.k0 && key < u.k1);
+    };
+    // Starts the loads of tile t of K or V into LDS.  Keys that are not there
+    // become zeros: neither their stale rows nor other pages' are read.
+    auto load = [&](int t, int page, uint64_t there, const char *base, char *to, int c0, int c1) {
+      const int key0 = t << kChunkTileShift;
+      if (there == ~uint64_t(0) && whole_groups) {
+        // A load instruction's rows in one page: scalar addresses.
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int r0 = (j * 4 + wave) * RPI, key = key0 + r0;
+          const int pg = __builtin_amdgcn_readlane(page, r0), slot = key - p.page_div.div(key) * p.page_size;
+          const char *at = base + ((int64_t)pg * p.page_b + (int64_t)slot * p.tok_b);
+          const uint32_t voff = (uint32_t)(lane / CP) * (uint32_t)p.tok_b + (uint32_t)(j & 1 ? c1 : c0);
+          lds_load16(at + voff, to + (j * 4 + wave) * 1024);
+        }
+        return;
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int r = lrow + j * 4 * RPI, key = key0 + r;
+        const int pg = __shfl(page, r, 64), slot = key - p.page_div.div(key) * p.page_size;
+        const char *at = base + ((int64_t)pg * p.page_b + (int64_t)slot * p.tok_b);
+        if (!((there >> r) & 1)) at = reinterpret_cast<const char *>(paged_zero_row);
+        lds_load16(at + (j & 1 ? c1 : c0), to + (j * 4 + wave) * 1024);
+      }
+    };
+
+    // The lane's query rows, their last keys, and the wave's tokens.
+    uint4 qx[RG][KS];
+    int tok[RG];
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      int qt, qh;
+      const bool own = u.row((wave * RG + g) * 32 + row, qt, qh);
+      const char *qp = p.q + (own ? qt : u.row0) * p.q_t + (own ? qh : u.head0) * p.q_h + 16 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) qx[g][st] = load16(qp + 32 * st);
+      tok[g] = own ? qt - u.row0 : 0;
+    }
+    const bool active = wave * RG * 32 < u.tokens * u.gw;
+    const int tok_a = min(wave * RG * 32 / u.gw, u.tokens - 1);
+    const int tok_z = min(((wave + 1) * RG * 32 - 1) / u.gw, u.tokens - 1);
+
+    f32x16_t o[RG][ND] = {};
+    float m_run[RG], l_lane[RG];
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      m_run[g] = -INFINITY;
+      l_lane[g] = 0.f;
+    }
+
+    // Hidden keys' scores of tile t become -inf.
+    auto hide = [&](f32x16_t(&s)[RG][2], int t, uint64_t there) {
+      const int64_t key0 = (int64_t)t << kChunkTileShift;
+      const bool edge = key0 + 63 > u.last0 + tok_a || (p.sh.window > 0 && key0 <= u.last0 + tok_z - p.sh.window);
+      if (!edge && there == ~uint64_t(0)) return;
+#pragma unroll
+      for (int g = 0; g < RG; ++g) {
+        const int64_t hi = u.last0 + tok[g] + 1 - key0, lo = p.sh.window > 0 ? hi - p.sh.window : 0;
+        uint64_t v = hi >= 64 ? ~uint64_t(0) : hi <= 0 ? 0 : (uint64_t(1) << hi) - 1;
+        if (lo > 0) v &= lo >= 64 ? 0 : ~uint64_t(0) << lo;
+        v = (v & there) >> (4 * hf);
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          const uint32_t bits = (uint32_t)(v >> (32 * sub));
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!(bits & (1u << (8 * (i >> 2) + (i & 3))))) s[g][sub][i] = -INFINITY;
+        }
+      }
+    };
+    // Raises the running maxima (and rescales the sums) where a score exceeds
+    // them by more than 2^kPgSlack.
+    auto raise = [&](const float (&x)[RG]) {
+#pragma unroll
+      for (int g = 0; g < RG; ++g) {
+        if (!__ballot(x[g] * cc > m_run[g] + kPgSlack)) continue;
+        const float mt = half_wave_max(x[g]) * cc;
+        const float m_new = mt > m_run[g] + kPgSlack ? mt : m_run[g];
+        const float a = m_run[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[g] - m_new);
+        l_lane[g] *= a;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) o[g][dt] *= a;
+        m_run[g] = m_new;
+      }
+    };
+    auto k_op = [&](const char *kb, int i) {
+      return *reinterpret_cast<const uint4 *>(kb + (kaddr ^ ((i % KS) << 5)) + (i / KS) * 32 * CP * 16);
+    };
+    auto v_op = [&](const char *vb, int k, int dt) {
+      const char *at = vb + vaddr[dt] + 16 * k * CP * 16;
+      const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t *)at));
+      const uint2 hi =
+          __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t *)(at + 8 * CP * 16)));
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    };
+    auto top = [&](const f32x16_t(&s)[RG][2], int g) {
+      float x = s[g][0][0];
+#pragma unroll
+      for (int i = 1; i < 32; ++i) x = fmaxf(x, s[g][i >> 4][i & 15]);
+      return x;
+    };
+    auto arrived = [&] {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(kPgWaitAll);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+
+    // Tiles in flight: pages (and presence) of tiles t + 1 .. t + 3.
+    int pg0 = lookup(part.t0), pg1 = lookup(part.t0 + 1), pg2 = lookup(part.t0 + 2);
+    uint64_t th0 = present(part.t0, pg0), th1 = present(part.t0 + 1, pg1);
+    load(part.t0, pg0, th0, kbase, kb0, kc0, kc1);
+    load(part.t0, pg0, th0, vbase, vb0, vc, vc);
+    if (part.t0 + 1 < part.t1) load(part.t0 + 1, pg1, th1, kbase, kb1, kc0, kc1);
+    arrived();
+    f32x16_t sa[RG][2] = {}, sb[RG][2];
+    if (active) {
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) {
+        const uint4 a = k_op(kb0, i);
+#pragma unroll
+        for (int g = 0; g < RG; ++g) sa[g][i / KS] = mfma_32x32x16<DT>(a, qx[g][i % KS], sa[g][i / KS]);
+      }
+      hide(sa, part.t0, th0);
+      float x[RG];
+#pragma unroll
+      for (int g = 0; g < RG; ++g) x[g] = top(sa, g);
+      raise(x);
+    }
+    int t = part.t0;
+    // One tile: sc its scores, vr its values; sn, kr the next tile's; kw, vw
+    // the buffers of the tiles behind those.
+    auto step = [&](f32x16_t(&sc)[RG][2], f32x16_t(&sn)[RG][2], const char *kr, const char *vr, char *kw, char *vw) {
+      if (t > part.t0) arrived();
+      else __syncthreads();  // every wave has read its K operands of the first tile
+      const uint64_t th2 = present(t + 2, pg2);
+      if (t + 2 < part.t1) load(t + 2, pg2, th2, kbase, kw, kc0, kc1);
+      if (t + 1 < part.t1) load(t + 1, pg1, th1, vbase, vw, vc, vc);
+      const int pg3 = lookup(t + 3);
+      if (active) {
+        float m_neg[RG];
+        uint4 pb[RG][4];
+#pragma unroll
+        for (int g = 0; g < RG; ++g) m_neg[g] = m_run[g] == -INFINITY ? 0.f : -m_run[g];
+        // Scores of the next tile (of no tile behind the last: not used)
+        // beside this one's probabilities, 2^(cc s - m), rounded to the dtype
+        // as operands; their sums keep the fp32 values.
+        constexpr int NR = 2 * KS, kAhead = NR < 4 ? NR : 4, PAIRS = 16 * RG;  // pairs of a lane's scores
+        uint4 ka[NR];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ka[i] = k_op(kr, i);
+        uint32_t w[RG][16];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+          if (i + kAhead < NR) ka[i + kAhead] = k_op(kr, i + kAhead);
+#pragma unroll
+          for (int g = 0; g < RG; ++g)
+            sn[g][i / KS] = mfma_32x32x16<DT>(ka[i], qx[g][i % KS], i % KS == 0 ? f32x16_t{} : sn[g][i / KS]);
+#pragma unroll
+          for (int e = PAIRS * i / NR; e < PAIRS * (i + 1) / NR; ++e) {
+            const int g = e >> 4, at = 2 * (e & 15);
+            const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[g][at >> 4][at & 15], cc, m_neg[g]));
+            const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[g][at >> 4][(at & 15) + 1], cc, m_neg[g]));
+            l_lane[g] += e0;
+            l_lane[g] += e1;
+            w[g][e & 15] = pack2<DT>(e0, e1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int g = 0; g < RG; ++g)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) pb[g][k] = make_uint4(w[g][4 * k], w[g][4 * k + 1], w[g][4 * k + 2], w[g][4 * k + 3]);
+        uint4 va[2][ND];
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) va[0][dt] = v_op(vr, 0, dt);
+        if (t + 1 < part.t1) hide(sn, t + 1, th1);
+        float x[RG];
+#pragma unroll
+        for (int g = 0; g < RG; ++g) x[g] = sn[g][0][0];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) {
+            if (k < 3) va[(k + 1) & 1][dt] = v_op(vr, k + 1, dt);
+#pragma unroll
+            for (int g = 0; g < RG; ++g) o[g][dt] = mfma_32x32x16<DT>(va[k & 1][dt], pb[g][k], o[g][dt]);
+          }
+#pragma unroll
+          for (int g = 0; g < RG; ++g)
+#pragma unroll
+            for (int i = 8 * k; i < 8 * k + 8; ++i) x[g] = fmaxf(x[g], sn[g][i >> 4][i & 15]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (t + 1 < part.t1) raise(x);
+      }
+      ++t;
+      pg1 = pg2;
+      th1 = th2;
+      pg2 = pg3;
+    };
+    while (t < part.t1) {
+      step(sa, sb, kb1, vb0, kb0, vb1);
+      if (t >= part.t1) break;
+      step(sb, sa, kb0, vb1, kb1, vb0);
+    }
+
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      const float l_row = half_wave_sum(l_lane[g]);
+      int qt, qh;
+      if (!u.row((wave * RG + g) * 32 + row, qt, qh)) continue;
+      if (part.partial >= 0) {
+        const int64_t sr = (int64_t)part.partial * p.sh.rows + (wave * RG + g) * 32 + row;
+        float *po = p.ws_o + sr * D + 4 * hf;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            *reinterpret_cast<f32x4_t *>(po + 32 * dt + 8 * n) =
+                f32x4_t{o[g][dt][4 * n], o[g][dt][4 * n + 1], o[g][dt][4 * n + 2], o[g][dt][4 * n + 3]};
+        if (hf == 0) {
+          p.ws_m[sr] = m_run[g];
+          p.ws_l[sr] = l_row;
+        }
+      } else {
+        // A row that sees no key gets zeros.
+        const float inv = l_row > 0.f ? 1.f / l_row : 0.f;
+        const int64_t at = ((int64_t)qt * p.hq + qh) * D + 4 * hf;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            store4<DT>(p.out, at + 32 * dt + 8 * n,
+                       f32x4_t{o[g][dt][4 * n], o[g][dt][4 * n + 1], o[g][dt][4 * n + 2], o[g][dt][4 * n + 3]} * inv);
+      }
+    }
+    if (wk.w < wk.w_end) {
+      __syncthreads();  // the next unit's first loads reuse the LDS
+      wk.next(p);
+    }
+  }
+}
+
 // Merges the units that the shares cut: o = sum_i 2^(m_i - M) o_i / sum_i
 // 2^(m_i - M) l_i over a unit's partial rows, M the largest of their maxima.
 // Grid (shares, rows / 4): one wave a row, its lanes D / 4 dims wide times the
@@ -588,8 +919,12 @@ template <int DT> __global__ void __launch_bounds__(kPgThreads) paged_combine_ke
 struct PagedPlan {
   PagedShape sh;
   int blocks, least;
+  bool chunk;  // the chunk kernel
   size_t m_off, l_off, o_off, total;  // workspace: cuts, then these
 };
+
+constexpr int chunk_groups(int D) { return D <= 128 ? 2 : 1; }  // row groups a wave's registers hold
+constexpr int chunk_rows(int D) { return 128 * chunk_groups(D); }
 
 static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
   const kiv_paged_cache_t &c = a.cache;
@@ -597,7 +932,9 @@ static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
   PagedPlan w;
   const int G = a.num_q_heads / c.num_kv_heads, cap = b.table_width * c.page_size;
   const int64_t most_keys = std::min<int64_t>(b.max_kv_len, cap);
-  const int rows = kRowsOfUnit, shift = kRowsTileShift;
+  // More rows of a kv head than a unit of the rows kernel has: the chunk kernel.
+  w.chunk = c.dtype != KIV_DTYPE_F32 && (int64_t)std::min(b.max_q_len, b.total_q) * G > kRowsOfUnit;
+  const int rows = w.chunk ? chunk_rows(c.head_dim) : kRowsOfUnit, shift = w.chunk ? kChunkTileShift : kRowsTileShift;
   w.sh = PagedShape::of(b.total_q, c.num_kv_heads, G, rows, cap, shift, a.window, false);
   // More than the call's units and tiles, by what the host knows of them.
   const int64_t units =
@@ -605,7 +942,8 @@ static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
   const int64_t keys = a.window > 0 ? std::min<int64_t>(most_keys, (int64_t)a.window + w.sh.tpu) : most_keys;
   const int64_t tiles = (keys >> shift) + 2;
   w.least = 1;
-  w.blocks = (int)std::max<int64_t>(8, std::min<int64_t>(2 * device_cu_count(), units * tiles) & ~int64_t(7));
+  const int slots = device_cu_count() * (w.chunk ? 1 : 2);
+  w.blocks = (int)std::max<int64_t>(8, std::min<int64_t>(slots, units * tiles) & ~int64_t(7));
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   const size_t parts = (size_t)2 * w.blocks * rows;
   w.m_off = up(w.blocks * sizeof(PagedCut));
@@ -706,7 +1044,11 @@ int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream
     const dim3 grid((unsigned)p.blocks), cgrid((unsigned)p.blocks, (unsigned)((p.sh.rows + kPgWaves - 1) / kPgWaves));
     auto go = [&](auto dtc) {
       constexpr int DTV = decltype(dtc)::value;
-      hipLaunchKernelGGL((paged_rows_kernel<DTV, DV>), grid, dim3(kPgThreads), 0, st, p);
+      if constexpr (DTV != DT_F32) {
+        if (w.chunk)
+          hipLaunchKernelGGL((paged_chunk_kernel<DTV, DV / 32, chunk_groups(DV)>), grid, dim3(kPgThreads), 0, st, p);
+      }
+      if (!w.chunk) hipLaunchKernelGGL((paged_rows_kernel<DTV, DV>), grid, dim3(kPgThreads), 0, st, p);
       hipLaunchKernelGGL((paged_combine_kernel<DTV>), cgrid, dim3(kPgThreads), 0, st, p, D);
     };
     if (c.dtype == KIV_DTYPE_F32) go(std::integral_constant<int, DT_F32>{});
