@@ -550,14 +550,14 @@ template <int DT, int KT, int RG> struct ChunkGeom {
 };
 constexpr int kChunkTileShift = 6;
 constexpr int kPgWaitAll = 0x0070;  // s_waitcnt vmcnt(0) lgkmcnt(0)
-typedef __attribute__((address_space(1))) const void gbl_void_t;
 
-__device__ __forceinline__ void lds_load16(const char *from, char *to) {
-  __builtin_amdgcn_global_load_lds((gbl_void_t *)from, (lds_void_t *)to, 16, 0, 0);
-}
+// Keeps x's computation where it is written: the compiler otherwise moves it
+// behind the next branch, to where x is used, and with it the vector
+// instructions that are to issue between matrix instructions.
+template <typename T> __device__ __forceinline__ void stay(T &x) { asm volatile("" : "+v"(x)); }
 
 template <int DT, int KT, int RG>
-__global__ void __launch_bounds__(kPgThreads, 1) paged_chunk_kernel(PagedAttnParams p) {
+__global__ void __launch_bounds__(kPgThreads, KT <= 4 ? 2 : 1) paged_chunk_kernel(PagedAttnParams p) {
   using Geo = ChunkGeom<DT, KT, RG>;
   constexpr int D = Geo::D, CP = Geo::CP, CPR = Geo::CPR, RPI = Geo::RPI, NJ = Geo::NJ, KS = Geo::KS, ND = Geo::ND;
   // Objects of their own, so that the compiler knows that reads of one do not
@@ -574,8 +574,9 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_chunk_kernel(PagedAttnPar
   // 4 RPI rows on) and its chunks' bytes; with 32 chunks the rows' K
   // permutation alternates.
   const int lrow = wave * RPI + lane / CP, pc = lane % CP;
-  const int kc0 = min(pc ^ Geo::xk(lrow), CPR - 1) * 16, kc1 = min(pc ^ Geo::xk(lrow + 4 * RPI), CPR - 1) * 16;
-  const int vc = min(pc ^ (4 * Geo::xv(lrow)), CPR - 1) * 16;
+  const uint32_t in_group = (uint32_t)(lane / CP) * (uint32_t)p.tok_b;  // the lane's row from its group's first
+  const uint32_t kc0 = min(pc ^ Geo::xk(lrow), CPR - 1) * 16, kc1 = min(pc ^ Geo::xk(lrow + 4 * RPI), CPR - 1) * 16;
+  const uint32_t vc = min(pc ^ (4 * Geo::xv(lrow)), CPR - 1) * 16;
   // Operand reads: the lane's byte offsets within a tile.
   const int kaddr = row * CP * 16 + ((hf ^ Geo::xk(row)) << 4);
   int vaddr[ND];
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_chunk_kernel(PagedAttnPar
     const int c = 4 * (dt ^ Geo::xv(q)) + 2 * ((lane >> 4) & 1) + ((j16 & 3) >> 1);
     vaddr[dt] = (4 * hf + q) * CP * 16 + c * 16 + (j16 & 1) * 8;
   }
-  const bool whole_groups = p.page_size % RPI == 0;  // a load instruction's rows lie in one page
+  const bool one_page = p.page_size % 64 == 0;  // a tile lies in one page
   const float cc = p.scale_log2;
   bool head = true;
   while (wk.w < wk.w_end) {
@@ -601,34 +602,51 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_chunk_kernel(PagedAttnPar
       const int key = (t << kChunkTileShift) + lane;
       return t < part.t1 && key < p.sh.cap ? table[p.page_div.div(key)] : -1;
     };
-    // Which of them are there (and seen by some row of the unit).
-    auto present = [&](int t, int page) {
-      const int key = (t << kChunkTileShift) + lane;
-      return __ballot(page >= 0 && page < p.num_pages && key >= u.k0 && key < u.k1);
+    // Where those keys' rows lie in the pool, a key a lane, and which of them
+    // are there (and seen by some row of the unit).
+    auto locate = [&](int t, int page, int64_t &off, uint64_t &there) {
+      const int key = (t << kChunkTileShift) + lane, slot = key - p.page_div.div(key) * p.page_size;
+      off = (int64_t)page * p.page_b + (int64_t)slot * p.tok_b;
+      there = __ballot(page >= 0 && page < p.num_pages && key >= u.k0 && key < u.k1);
     };
-    // Starts the loads of tile t of K or V into LDS.  Keys that are not there
-    // become zeros: neither their stale rows nor other pages' are read.
-    auto load = [&](int t, int page, uint64_t there, const char *base, char *to, int c0, int c1) {
-      const int key0 = t << kChunkTileShift;
-      if (there == ~uint64_t(0) && whole_groups) {
-        // A load instruction's rows in one page: scalar addresses.
+    // Starts the loads of a tile of K or V into LDS: a load instruction's rows
+    // lie in one page, so its addresses are that page's (in scalar registers)
+    // and the lanes' fixed offsets.  Keys that are not there are given the row
+    // of one that is (zeros if there is none): neither their stale rows nor
+    // other sequences' are read.
+    auto load = [&](int64_t off, uint64_t there, const char *base, char *to, uint32_t c0, uint32_t c1) {
+      auto row_at = [&](int r) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)off, r);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(off >> 32), r);
+        return tile_rsrc(base + (int64_t)((uint64_t)hi << 32 | lo), 0xffffffffu);
+      };
+      auto put = [&](__amdgpu_buffer_rsrc_t rs, int j, uint32_t voff, uint32_t soff) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t *)(to + (j * 4 + wave) * 1024), 16,
+                                                 (int)(voff + (j & 1 ? c1 : c0)), (int)soff, 0, 0);
+      };
+      if (there == ~uint64_t(0)) {
+        if (one_page) {
+          const auto rs = row_at(0);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const int r0 = (j * 4 + wave) * RPI, key = key0 + r0;
-          const int pg = __builtin_amdgcn_readlane(page, r0), slot = key - p.page_div.div(key) * p.page_size;
-          const char *at = base + ((int64_t)pg * p.page_b + (int64_t)slot * p.tok_b);
-          const uint32_t voff = (uint32_t)(lane / CP) * (uint32_t)p.tok_b + (uint32_t)(j & 1 ? c1 : c0);
-          lds_load16(at + voff, to + (j * 4 + wave) * 1024);
+          for (int j = 0; j < NJ; ++j) put(rs, j, in_group, (uint32_t)((j * 4 + wave) * RPI) * (uint32_t)p.tok_b);
+        } else {
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) put(row_at((j * 4 + wave) * RPI), j, in_group, 0);
         }
         return;
       }
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const int r = lrow + j * 4 * RPI, key = key0 + r;
-        const int pg = __shfl(page, r, 64), slot = key - p.page_div.div(key) * p.page_size;
-        const char *at = base + ((int64_t)pg * p.page_b + (int64_t)slot * p.tok_b);
-        if (!((there >> r) & 1)) at = reinterpret_cast<const char *>(paged_zero_row);
-        lds_load16(at + (j & 1 ? c1 : c0), to + (j * 4 + wave) * 1024);
+        const int r0 = (j * 4 + wave) * RPI;
+        const uint32_t in = (uint32_t)(there >> r0) & ((1u << RPI) - 1u);  // of the group: consecutive
+        if (in) {
+          const int lo = __builtin_ctz(in), hi = 31 - __builtin_clz(in);
+          put(row_at(r0 + lo), j, (uint32_t)(min(max(lane / CP, lo), hi) - lo) * (uint32_t)p.tok_b, 0);
+        } else if (there) {
+          put(row_at(__builtin_ctzll(there)), j, 0, 0);
+        } else {
+          put(tile_rsrc(reinterpret_cast<const char *>(paged_zero_row), 0xffffffffu), j, 0, 0);
+        }
       }
     };
 
@@ -715,12 +733,15 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_chunk_kernel(PagedAttnPar
       asm volatile("" ::: "memory");
     };
 
-    // Tiles in flight: pages (and presence) of tiles t + 1 .. t + 3.
+    // In flight: where tile t + 1's keys lie, the pages of tile t + 2's.
     int pg0 = lookup(part.t0), pg1 = lookup(part.t0 + 1), pg2 = lookup(part.t0 + 2);
-    uint64_t th0 = present(part.t0, pg0), th1 = present(part.t0 + 1, pg1);
-    load(part.t0, pg0, th0, kbase, kb0, kc0, kc1);
-    load(part.t0, pg0, th0, vbase, vb0, vc, vc);
-    if (part.t0 + 1 < part.t1) load(part.t0 + 1, pg1, th1, kbase, kb1, kc0, kc1);
+    int64_t off0, off1;
+    uint64_t th0, th1;
+    locate(part.t0, pg0, off0, th0);
+    load(off0, th0, kbase, kb0, kc0, kc1);
+    load(off0, th0, vbase, vb0, vc, vc);
+    locate(part.t0 + 1, pg1, off1, th1);
+    if (part.t0 + 1 < part.t1) load(off1, th1, kbase, kb1, kc0, kc1);
     arrived();
     f32x16_t sa[RG][2] = {}, sb[RG][2];
     if (active) {
@@ -740,11 +761,13 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_chunk_kernel(PagedAttnPar
     // One tile: sc its scores, vr its values; sn, kr the next tile's; kw, vw
     // the buffers of the tiles behind those.
     auto step = [&](f32x16_t(&sc)[RG][2], f32x16_t(&sn)[RG][2], const char *kr, const char *vr, char *kw, char *vw) {
-      if (t > part.t0) arrived();
-      else __syncthreads();  // every wave has read its K operands of the first tile
-      const uint64_t th2 = present(t + 2, pg2);
-      if (t + 2 < part.t1) load(t + 2, pg2, th2, kbase, kw, kc0, kc1);
-      if (t + 1 < part.t1) load(t + 1, pg1, th1, vbase, vw, vc, vc);
+      arrived();
+      // The pages' numbers first: behind new loads they would wait for those.
+      int64_t off2;
+      uint64_t th2;
+      locate(t + 2, pg2, off2, th2);
+      if (t + 1 < part.t1) load(off1, th1, vbase, vw, vc, vc);
+      if (t + 2 < part.t1) load(off2, th2, kbase, kw, kc0, kc1);
       const int pg3 = lookup(t + 3);
       if (active) {
         float m_neg[RG];
@@ -754,7 +777,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_chunk_kernel(PagedAttnPar
         // Scores of the next tile (of no tile behind the last: not used)
         // beside this one's probabilities, 2^(cc s - m), rounded to the dtype
         // as operands; their sums keep the fp32 values.
-        constexpr int NR = 2 * KS, kAhead = NR < 4 ? NR : 4, PAIRS = 16 * RG;  // pairs of a lane's scores
+        constexpr int NR = 2 * KS, kAhead = NR < 3 ? NR : 3, PAIRS = 16 * RG;  // pairs of a lane's scores
         uint4 ka[NR];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) ka[i] = k_op(kr, i);
@@ -773,38 +796,40 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_chunk_kernel(PagedAttnPar
             l_lane[g] += e0;
             l_lane[g] += e1;
             w[g][e & 15] = pack2<DT>(e0, e1);
+            stay(w[g][e & 15]);
           }
+#pragma unroll
+          for (int g = 0; g < RG; ++g) stay(l_lane[g]);
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int g = 0; g < RG; ++g)
 #pragma unroll
           for (int k = 0; k < 4; ++k) pb[g][k] = make_uint4(w[g][4 * k], w[g][4 * k + 1], w[g][4 * k + 2], w[g][4 * k + 3]);
-        uint4 va[2][ND];
+        constexpr int NV = 4 * ND, vAhead = NV < 4 ? NV : 4;
+        uint4 va[NV];
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt) va[0][dt] = v_op(vr, 0, dt);
+        for (int i = 0; i < vAhead; ++i) va[i] = v_op(vr, i / ND, i % ND);
         if (t + 1 < part.t1) hide(sn, t + 1, th1);
         float x[RG];
 #pragma unroll
         for (int g = 0; g < RG; ++g) x[g] = sn[g][0][0];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int i = 0; i < NV; ++i) {
+          if (i + vAhead < NV) va[i + vAhead] = v_op(vr, (i + vAhead) / ND, (i + vAhead) % ND);
 #pragma unroll
-          for (int dt = 0; dt < ND; ++dt) {
-            if (k < 3) va[(k + 1) & 1][dt] = v_op(vr, k + 1, dt);
+          for (int g = 0; g < RG; ++g) {
+            o[g][i % ND] = mfma_32x32x16<DT>(va[i], pb[g][i / ND], o[g][i % ND]);
 #pragma unroll
-            for (int g = 0; g < RG; ++g) o[g][dt] = mfma_32x32x16<DT>(va[k & 1][dt], pb[g][k], o[g][dt]);
+            for (int e = 32 * i / NV; e < 32 * (i + 1) / NV; ++e) x[g] = fmaxf(x[g], sn[g][e >> 4][e & 15]);
+            stay(x[g]);
           }
-#pragma unroll
-          for (int g = 0; g < RG; ++g)
-#pragma unroll
-            for (int i = 8 * k; i < 8 * k + 8; ++i) x[g] = fmaxf(x[g], sn[g][i >> 4][i & 15]);
           __builtin_amdgcn_sched_barrier(0);
         }
         if (t + 1 < part.t1) raise(x);
       }
       ++t;
-      pg1 = pg2;
+      off1 = off2;
       th1 = th2;
       pg2 = pg3;
     };
@@ -853,66 +878,92 @@ __global__ void __launch_bounds__(kPgThreads, 1) paged_chunk_kernel(PagedAttnPar
 
 // Merges the units that the shares cut: o = sum_i 2^(m_i - M) o_i / sum_i
 // 2^(m_i - M) l_i over a unit's partial rows, M the largest of their maxima.
-// Grid (shares, rows / 4): one wave a row, its lanes D / 4 dims wide times the
-// parts side by side; blocks of shares that continue no unit leave at once.
-constexpr int kCombineParts = 4;  // parts of a lane in flight together
-template <int DT> __global__ void __launch_bounds__(kPgThreads) paged_combine_kernel(PagedAttnParams p, int D) {
-  const int id = blockIdx.x;
-  const PagedCut c = p.cuts[id];
-  if (c.last < 0) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int r = blockIdx.y * kPgWaves + wave, gw = p.sh.gw, tok = r / gw, g = r - tok * gw;
-  if (r >= p.sh.rows || tok >= c.tokens || g >= c.heads) return;
-  const int n = c.last - id + 2;  // the part of the block before, then parts id .. last
-  const int wide = D / 4 <= 64 ? D / 4 : 64, side = 64 / wide, mine = lane / wide, d0 = 4 * (lane - mine * wide);
-  auto at = [&](int i) { return (int64_t)(i == 0 ? 2 * id - 1 : 2 * (id + i - 1)) * p.sh.rows + r; };
-  float M = -INFINITY, L = 0.f;
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-  if (mine < side) {
-    for (int i0 = mine; i0 < n; i0 += kCombineParts * side) {
-      float ms[kCombineParts], ls[kCombineParts];
-      f32x4_t os[kCombineParts];
+// A block takes the cuts of neighbouring shares; D / 4 threads a row, kCombineParts
+// parts of it in flight together.  SPLIT (units cut into many parts): a row a
+// block, its parts dealt to the block's groups of D / 4 threads, whose sums
+// meet in LDS; else a row a group.
+constexpr int kCombineParts = 4;
+struct PartialSum {
+  float m = -INFINITY, l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+};
+// Parts first, first + step, ... < n of row r of the unit cut in front of block id.
+__device__ __forceinline__ PartialSum paged_sum_parts(const PagedAttnParams &p, int D, int id, int r, int d0, int n,
+                                                      int first, int step) {
+  PartialSum s;
+  for (int i0 = first; i0 < n; i0 += kCombineParts * step) {
+    float ms[kCombineParts], ls[kCombineParts];
+    f32x4_t os[kCombineParts];
 #pragma unroll
-      for (int k = 0; k < kCombineParts; ++k) {
-        const bool in = i0 + k * side < n;
-        const int64_t x = at(in ? i0 + k * side : i0);
-        ms[k] = in ? p.ws_m[x] : -INFINITY;
-        ls[k] = in ? p.ws_l[x] : 0.f;
-        os[k] = *reinterpret_cast<const f32x4_t *>(p.ws_o + x * D + d0);
+    for (int k = 0; k < kCombineParts; ++k) {
+      const bool in = i0 + k * step < n;
+      const int i = in ? i0 + k * step : i0;
+      const int64_t x = (int64_t)(i == 0 ? 2 * id - 1 : 2 * (id + i - 1)) * p.sh.rows + r;
+      ms[k] = in ? p.ws_m[x] : -INFINITY;
+      ls[k] = in ? p.ws_l[x] : 0.f;
+      os[k] = *reinterpret_cast<const f32x4_t *>(p.ws_o + x * D + d0);
+    }
+    float m = s.m;
+#pragma unroll
+    for (int k = 0; k < kCombineParts; ++k) m = fmaxf(m, ms[k]);
+    if (m == -INFINITY) continue;
+    const float a = s.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s.m - m);
+    s.l *= a;
+    s.o *= a;
+#pragma unroll
+    for (int k = 0; k < kCombineParts; ++k) {
+      const float w = ms[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[k] - m);
+      s.l = fmaf(w, ls[k], s.l);
+      s.o += w * os[k];
+    }
+    s.m = m;
+  }
+  return s;
+}
+
+template <int DT, bool SPLIT>
+__global__ void __launch_bounds__(kPgThreads) paged_combine_kernel(PagedAttnParams p, int D) {
+  __shared__ float gm[kPgThreads], gl[kPgThreads];
+  __shared__ f32x4_t go[kPgThreads];
+  const int tid = threadIdx.x, lane = tid & 63, wide = D / 4, groups = kPgThreads / wide;
+  const int group = tid / wide, d0 = 4 * (tid - group * wide), gw = p.sh.gw;
+  const int per = (p.blocks + gridDim.x - 1) / gridDim.x, end = min((int)(blockIdx.x + 1) * per, p.blocks);
+  for (int base = blockIdx.x * per; base < end; base += 64) {
+    for (uint64_t cut = __ballot(base + lane < end && p.cuts[min(base + lane, end - 1)].last >= 0); cut;
+         cut &= cut - 1) {
+      const int id = base + __builtin_ctzll(cut);
+      const PagedCut c = p.cuts[id];
+      const int n = c.last - id + 2;  // the part of the block before, then parts id .. last
+      const int rows = c.tokens * gw;
+      for (int r0 = blockIdx.y * (SPLIT ? 1 : groups); r0 < rows; r0 += gridDim.y * (SPLIT ? 1 : groups)) {
+        const int r = SPLIT ? r0 : r0 + group, tok = r / gw, g = r - tok * gw;
+        const bool own = group < groups && r < rows && g < c.heads;
+        if (SPLIT && r % gw >= c.heads) continue;
+        PartialSum s;
+        if (own) s = paged_sum_parts(p, D, id, r, d0, n, SPLIT ? group : 0, SPLIT ? groups : 1);
+        if constexpr (SPLIT) {
+          __syncthreads();
+          gm[tid] = s.m;
+          gl[tid] = s.l;
+          go[tid] = s.o;
+          __syncthreads();
+          if (group != 0) continue;
+          float M = s.m;
+          for (int k = 1; k < groups; ++k) M = fmaxf(M, gm[tid + k * wide]);
+          PartialSum all;
+          for (int k = 0; k < groups; ++k) {
+            const float m = gm[tid + k * wide], w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+            all.l = fmaf(w, gl[tid + k * wide], all.l);
+            all.o += w * go[tid + k * wide];
+          }
+          s = all;
+        }
+        if (!own) continue;
+        const float inv = s.l > 0.f ? 1.f / s.l : 0.f;
+        store4<DT>(p.out, ((int64_t)(c.row0 + tok) * p.hq + c.head0 + g) * D + d0, s.o * inv);
       }
-      float m = M;
-#pragma unroll
-      for (int k = 0; k < kCombineParts; ++k) m = fmaxf(m, ms[k]);
-      if (m == -INFINITY) continue;
-      const float a = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m);
-      L *= a;
-      acc *= a;
-#pragma unroll
-      for (int k = 0; k < kCombineParts; ++k) {
-        const float w = ms[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[k] - m);
-        L = fmaf(w, ls[k], L);
-        acc += w * os[k];
-      }
-      M = m;
     }
   }
-  // The sides' sums: lane mine * wide + d adds those of the other sides.
-  float MM = M;
-  for (int k = 1; k < side; ++k) MM = fmaxf(MM, __shfl(M, (lane + k * wide) % (side * wide), 64));
-  const float a = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - MM);
-  L *= a;
-  acc *= a;
-  float LL = L;
-  f32x4_t sum = acc;
-  for (int k = 1; k < side; ++k) {
-    const int from = (lane + k * wide) % (side * wide);
-    LL += __shfl(L, from, 64);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] += __shfl(acc[j], from, 64);
-  }
-  if (mine != 0) return;
-  const float inv = LL > 0.f ? 1.f / LL : 0.f;
-  store4<DT>(p.out, ((int64_t)(c.row0 + tok) * p.hq + c.head0 + g) * D + d0, sum * inv);
 }
 
 // ------------------------------------------------------------------- host
@@ -920,10 +971,13 @@ struct PagedPlan {
   PagedShape sh;
   int blocks, least;
   bool chunk;  // the chunk kernel
+  bool split;  // units are cut into many parts
+  int cuts_x, cuts_y;  // the combine's grid
   size_t m_off, l_off, o_off, total;  // workspace: cuts, then these
 };
 
-constexpr int chunk_groups(int D) { return D <= 128 ? 2 : 1; }  // row groups a wave's registers hold
+constexpr int chunk_groups(int D) { return 1; }
+constexpr int chunk_load_rows(int D) { return D <= 32 ? 16 : D <= 64 ? 8 : D <= 128 ? 4 : 2; }
 constexpr int chunk_rows(int D) { return 128 * chunk_groups(D); }
 
 static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
@@ -932,8 +986,11 @@ static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
   PagedPlan w;
   const int G = a.num_q_heads / c.num_kv_heads, cap = b.table_width * c.page_size;
   const int64_t most_keys = std::min<int64_t>(b.max_kv_len, cap);
-  // More rows of a kv head than a unit of the rows kernel has: the chunk kernel.
-  w.chunk = c.dtype != KIV_DTYPE_F32 && (int64_t)std::min(b.max_q_len, b.total_q) * G > kRowsOfUnit;
+  // More rows of a kv head than a unit of the rows kernel has: the chunk
+  // kernel, if the rows of one of its load instructions lie in one page and
+  // a tile's rows within 2 GiB.
+  w.chunk = c.dtype != KIV_DTYPE_F32 && (int64_t)std::min(b.max_q_len, b.total_q) * G > kRowsOfUnit &&
+            c.page_size % chunk_load_rows(c.head_dim) == 0 && c.stride[2] >= 0 && c.stride[2] < (1 << 24);
   const int rows = w.chunk ? chunk_rows(c.head_dim) : kRowsOfUnit, shift = w.chunk ? kChunkTileShift : kRowsTileShift;
   w.sh = PagedShape::of(b.total_q, c.num_kv_heads, G, rows, cap, shift, a.window, false);
   // More than the call's units and tiles, by what the host knows of them.
@@ -942,8 +999,13 @@ static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
   const int64_t keys = a.window > 0 ? std::min<int64_t>(most_keys, (int64_t)a.window + w.sh.tpu) : most_keys;
   const int64_t tiles = (keys >> shift) + 2;
   w.least = 1;
-  const int slots = device_cu_count() * (w.chunk ? 1 : 2);
+  const int slots = device_cu_count() * (w.chunk && c.head_dim > 128 ? 1 : 2);
   w.blocks = (int)std::max<int64_t>(8, std::min<int64_t>(slots, units * tiles) & ~int64_t(7));
+  w.split = w.blocks > 6 * units;
+  w.cuts_x = (int)std::min<int64_t>(w.blocks, std::max<int64_t>(1, units));
+  const int most_rows = (int)std::min<int64_t>(rows, (int64_t)w.sh.gw * std::max(1, std::min(w.sh.tpu, b.max_q_len)));
+  const int groups = kPgThreads / (c.head_dim / 4);
+  w.cuts_y = w.split ? most_rows : (most_rows + 2 * groups - 1) / (2 * groups);
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   const size_t parts = (size_t)2 * w.blocks * rows;
   w.m_off = up(w.blocks * sizeof(PagedCut));
@@ -1041,7 +1103,7 @@ int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream
   const int D = c.head_dim;
   return with_head_dim(D, [&](auto dc) {
     constexpr int DV = decltype(dc)::value;
-    const dim3 grid((unsigned)p.blocks), cgrid((unsigned)p.blocks, (unsigned)((p.sh.rows + kPgWaves - 1) / kPgWaves));
+    const dim3 grid((unsigned)p.blocks), cgrid((unsigned)w.cuts_x, (unsigned)w.cuts_y);
     auto go = [&](auto dtc) {
       constexpr int DTV = decltype(dtc)::value;
       if constexpr (DTV != DT_F32) {
@@ -1049,7 +1111,8 @@ int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream
           hipLaunchKernelGGL((paged_chunk_kernel<DTV, DV / 32, chunk_groups(DV)>), grid, dim3(kPgThreads), 0, st, p);
       }
       if (!w.chunk) hipLaunchKernelGGL((paged_rows_kernel<DTV, DV>), grid, dim3(kPgThreads), 0, st, p);
-      hipLaunchKernelGGL((paged_combine_kernel<DTV>), cgrid, dim3(kPgThreads), 0, st, p, D);
+      if (w.split) hipLaunchKernelGGL((paged_combine_kernel<DTV, true>), cgrid, dim3(kPgThreads), 0, st, p, D);
+      else hipLaunchKernelGGL((paged_combine_kernel<DTV, false>), cgrid, dim3(kPgThreads), 0, st, p, D);
     };
     if (c.dtype == KIV_DTYPE_F32) go(std::integral_constant<int, DT_F32>{});
     else if (c.dtype == KIV_DTYPE_F16) go(std::integral_constant<int, DT_F16>{});
