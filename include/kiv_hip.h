@@ -442,7 +442,7 @@ typedef struct {
 } kiv_paged_attention_args_t;
 
 /* Workspace bytes kiv_paged_attention needs for these arguments, with the
- * current device (0: refused arguments, or nothing to do). */
+ * current device (0: refused arguments, or none needed). */
 size_t kiv_paged_attention_workspace_size(const kiv_paged_attention_args_t *args);
 
 /* One softmax per packed row and head over the keys of its sequence up to its

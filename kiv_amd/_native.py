@@ -228,18 +228,55 @@ def mask_kind(dtype: torch.dtype) -> int:
         raise TypeError(f"unsupported attention mask dtype {dtype}") from None
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_entry: dict[str, object] = {}
+
+
 def call(name: str, args: C.Structure, device: torch.device) -> None:
     """Run entry point ``name`` on torch's current stream of ``device``, with
     that device current."""
-    fn = getattr(lib(), name)
-    if device.index == torch.cuda.current_device():
-        check(fn(C.byref(args), stream_ptr(device)), name)
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(lib(), name)
+    if device.index == _current_device():
+        rc = fn(args, stream_ptr(device))
     else:
         with torch.cuda.device(device):
-            check(fn(C.byref(args), stream_ptr(device)), name)
+            rc = fn(args, stream_ptr(device))
+    if rc:
+        check(rc, name)
 
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+class Layout:
+    """What the kernels need to know of a tensor's rows: the leading strides
+    as a ctypes array, and whether its rows can be loaded as they are (unit
+    stride over the last dimension, strides of whole 16-byte chunks)."""
+
+    __slots__ = ("strides", "chunked")
+
+    def __init__(self, shape, st, esize: int) -> None:
+        n = len(shape) - 1
+        lead = [0 if shape[i] == 1 else st[i] for i in range(n)]
+        self.strides = _ARRAYS.get(n, C.c_int64 * n)(*lead)
+        vec = 16 // esize
+        self.chunked = st[-1] == 1 and all(x % vec == 0 for x in lead)
+
+
+_layouts: dict[tuple, Layout] = {}
+
+
+def layout(t: torch.Tensor) -> Layout:
+    """The :class:`Layout` of t's shape and strides (shared between calls)."""
+    key = (t.shape, t.stride(), t.dtype)
+    got = _layouts.get(key)
+    if got is None:
+        got = Layout(key[0], key[1], t.element_size())
+        if len(_layouts) < 4096:
+            _layouts[key] = got
+    return got
 
 
 def stream_ptr(device: torch.device) -> int:

@@ -68,23 +68,24 @@ struct PagedAttnParams {
 // A row of zeros that stands for keys that are not there.
 __device__ const uint4 paged_zero_row[64] = {};
 
-// Tiles of a sequence's units of one kv head, by the whole wave (each lane
+__device__ __forceinline__ int uniform_i32(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Weight of a sequence's units of one kv head, by the whole wave (each lane
 // its own sequence; long ones by all lanes together).
-__device__ __forceinline__ int64_t paged_seq_weight(const PagedShape &sh, const PagedSeq &s) {
+__device__ __forceinline__ int paged_seq_weight(const PagedShape &sh, const PagedSeq &s) {
   const int nrt = sh.row_tiles(s);
   if (sh.whole) return nrt;
-  constexpr int kSerial = 4;
-  int64_t w = 0;
+  constexpr int kSerial = 2;
+  int w = 0;
   if (nrt <= kSerial)
     for (int rt = 0; rt < nrt; ++rt) w += sh.weight(s, rt);
   const int lane = threadIdx.x & 63;
   for (uint64_t m = __ballot(nrt > kSerial); m; m &= m - 1) {
-    const int l = __builtin_ctzll(m), n = __shfl(nrt, l, 64);
-    const PagedSeq o{0, __shfl(s.qlen, l, 64), __shfl(s.len, l, 64)};
-    int64_t sum = 0;
+    const int l = __builtin_ctzll(m), n = __builtin_amdgcn_readlane(nrt, l);
+    const PagedSeq o{0, __builtin_amdgcn_readlane(s.qlen, l), __builtin_amdgcn_readlane(s.len, l)};
+    int sum = 0;
     for (int rt = lane; rt < n; rt += 64) sum += sh.weight(o, rt);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    sum = wave_sum_i32(sum);
     if (lane == l) w = sum;
   }
   return w;
@@ -101,100 +102,117 @@ struct PagedWork {
   int b, kvh, rt;   // the unit
   PagedSeq s;
   int nrt;
-  int64_t w, w_end, us;  // the share's next weight and end; the unit's first weight
+  int w, w_end, us;  // the share's next weight and end; the unit's first weight
   PagedShares shares;
 
-  // Called by the whole block; false: there is no share for it.
+  // Called by the whole block; false: there is no share for it.  Up to 64
+  // sequences every wave sums for itself; more meet in LDS.
   __device__ __forceinline__ bool first(const PagedAttnParams &p) {
-    __shared__ int64_t sums[kPgWaves];
-    __shared__ int64_t found[3];
+    __shared__ int sums[kPgWaves], found[3];
+    __shared__ float fsums[kPgWaves];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const PagedShape &sh = p.sh;
-    // All weights: thread tid's sequence of each kPgThreads, and the block's
-    // sums of them.
-    int64_t mine = 0, total = 0, incl = 0;
-    for (int base = 0; base < p.seqs; base += kPgThreads) {
-      mine = sh.hkv * paged_seq_weight(sh, paged_seq(p, base + tid));
-      total += scan(mine, incl, sums, wave, lane);
+    int seq_at, seq_w;  // the sequence's first weight, and all of them
+    if (p.seqs <= 64) {
+      const PagedSeq my = paged_seq(p, lane);
+      const int mine = sh.hkv * paged_seq_weight(sh, my), incl = wave_incl_scan(mine);
+      if (!deal(p, __builtin_amdgcn_readlane(incl, 63), wave_sum((float)mine))) return false;
+      b = __builtin_ctzll(__ballot(incl > w));
+      seq_w = __builtin_amdgcn_readlane(mine, b);
+      seq_at = __builtin_amdgcn_readlane(incl, b) - seq_w;
+      s.q0 = __builtin_amdgcn_readlane(my.q0, b);
+      s.qlen = __builtin_amdgcn_readlane(my.qlen, b);
+      s.len = __builtin_amdgcn_readlane(my.len, b);
+    } else {
+      int mine = 0, incl = 0, total = 0;
+      float ftotal = 0.f;
+      for (int base = 0; base < p.seqs; base += kPgThreads) {
+        mine = sh.hkv * paged_seq_weight(sh, paged_seq(p, base + tid));
+        const float f = wave_sum((float)mine);
+        __syncthreads();
+        if (lane == 0) fsums[wave] = f;
+        total += scan(mine, incl, sums, wave, lane);
+#pragma unroll
+        for (int i = 0; i < kPgWaves; ++i) ftotal += fsums[i];
+      }
+      if (!deal(p, total, ftotal)) return false;
+      int before = 0;
+      for (int base = 0; base < p.seqs; base += kPgThreads) {
+        int sum = total;
+        if (p.seqs > kPgThreads) {
+          mine = sh.hkv * paged_seq_weight(sh, paged_seq(p, base + tid));
+          sum = scan(mine, incl, sums, wave, lane);
+        }
+        const int end = before + incl;
+        if (w < end && w >= end - mine) {
+          found[0] = base + tid;
+          found[1] = end - mine;
+          found[2] = mine;
+        }
+        before += sum;
+        if (w < before) break;
+      }
+      __syncthreads();
+      b = uniform_i32(found[0]);
+      seq_at = uniform_i32(found[1]);
+      seq_w = uniform_i32(found[2]);
+      load_seq(p);
     }
-    shares.total = total;
-    if (total == 0) return false;
-    shares.n = PagedShares::blocks(total, p.blocks, p.least);
+    nrt = sh.row_tiles(s);
+    const int per_head = seq_w / sh.hkv;
+    kvh = (w - seq_at) / per_head;
+    int r = w - seq_at - kvh * per_head;  // weights of the head's units before w
+    if (sh.whole) {
+      rt = r;
+      us = w;
+      return true;
+    }
+    for (rt = 0;; rt += 64) {
+      const int n = rt + lane < nrt ? sh.weight(s, rt + lane) : 0, up = wave_incl_scan(n);
+      const uint64_t past = __ballot(up > r);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        rt += l;
+        us = w - (r - (__builtin_amdgcn_readlane(up, l) - __builtin_amdgcn_readlane(n, l)));
+        return true;
+      }
+      r -= __builtin_amdgcn_readlane(up, 63);
+    }
+  }
+  // This block's share of `total` (ftotal: the same sum in floating point, by
+  // which lengths in disorder, whose sum passes 2^31, are known: a batch in
+  // order stays below by the host's check).
+  __device__ __forceinline__ bool deal(const PagedAttnParams &p, int total, float ftotal) {
+    if (total <= 0 || ftotal > 2.1e9f) return false;
+    shares = PagedShares::deal(total, p.blocks, p.least);
     if ((int)blockIdx.x >= shares.n) return false;
     // Blocks are dealt to the eight dies in turn: a die takes neighbouring
     // shares, which read the same keys through its L2.
     id = !(shares.n & 7) ? ((int)blockIdx.x & 7) * (shares.n >> 3) + ((int)blockIdx.x >> 3) : (int)blockIdx.x;
     w = shares.start(id);
     w_end = shares.start(id + 1);
-    // The sequence that weight w falls in.
-    int64_t before = 0;
-    for (int base = 0; base < p.seqs; base += kPgThreads) {
-      int64_t sum = total;
-      if (p.seqs > kPgThreads) {
-        mine = sh.hkv * paged_seq_weight(sh, paged_seq(p, base + tid));
-        sum = scan(mine, incl, sums, wave, lane);
-      }
-      const int64_t end = before + incl;
-      if (w < end && w >= end - mine) {
-        found[0] = base + tid;
-        found[1] = end - mine;
-        found[2] = mine;
-      }
-      before += sum;
-      if (w < before) break;
-    }
-    __syncthreads();
-    b = (int)uniform_i64(found[0]);
-    const int64_t in = w - uniform_i64(found[1]), per_head = uniform_i64(found[2]) / sh.hkv;
-    s = paged_seq(p, b);
-    nrt = sh.row_tiles(s);
-    kvh = (int)(in / per_head);
-    int64_t r = in - kvh * per_head;  // weights of the head's units before w
-    if (sh.whole) {
-      rt = (int)r;
-      us = w;
-      return true;
-    }
-    for (rt = 0;; rt += 64) {
-      int64_t up = rt + lane < nrt ? sh.weight(s, rt + lane) : 0;
-      const int64_t n = up;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int64_t t = __shfl_up(up, d, 64);
-        if (lane >= d) up += t;
-      }
-      const uint64_t past = __ballot(up > r);
-      if (past) {
-        const int l = __builtin_ctzll(past);
-        rt += l;
-        us = w - (r - (__shfl(up, l, 64) - __shfl(n, l, 64)));
-        break;
-      }
-      r -= __shfl(up, 63, 64);
-    }
-    rt = (int)uniform_u32((uint32_t)rt);
-    us = uniform_i64(us);
     return true;
   }
   // Inclusive sums over the block's threads; returns the block's.
-  static __device__ __forceinline__ int64_t scan(int64_t x, int64_t &incl, int64_t *sums, int wave, int lane) {
-    incl = x;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t t = __shfl_up(incl, d, 64);
-      if (lane >= d) incl += t;
-    }
+  static __device__ __forceinline__ int scan(int x, int &incl, int *sums, int wave, int lane) {
+    incl = wave_incl_scan(x);
     __syncthreads();
     if (lane == 63) sums[wave] = incl;
     __syncthreads();
-    int64_t all = 0;
+    int all = 0;
 #pragma unroll
     for (int i = 0; i < kPgWaves; ++i) {
-      const int64_t t = sums[i];
+      const int t = sums[i];
       if (i < wave) incl += t;
       all += t;
     }
-    return uniform_i64(all);
+    return uniform_i32(all);
+  }
+  __device__ __forceinline__ void load_seq(const PagedAttnParams &p) {
+    s = paged_seq(p, b);
+    s.q0 = uniform_i32(s.q0);
+    s.qlen = uniform_i32(s.qlen);
+    s.len = uniform_i32(s.len);
   }
   // The unit behind this one; called while w < w_end.
   __device__ __forceinline__ void next(const PagedAttnParams &p) {
@@ -205,10 +223,7 @@ struct PagedWork {
     kvh = 0;
     do {
       ++b;
-      s = paged_seq(p, b);
-      s.q0 = (int)uniform_u32(s.q0);
-      s.qlen = (int)uniform_u32(s.qlen);
-      s.len = (int)uniform_u32(s.len);
+      load_seq(p);
       nrt = p.sh.row_tiles(s);
     } while (nrt == 0 && b < p.seqs);
   }
@@ -218,7 +233,7 @@ struct PagedWork {
 struct PagedUnit {
   int row0, tokens, head0, heads;  // first packed row, tokens, first query head, heads
   int gw;
-  int64_t last0;   // last key that the first token sees
+  int last0;       // last key that the first token sees
   int k0, k1;      // keys that some row sees
   __device__ __forceinline__ PagedUnit(const PagedShape &sh, const PagedSeq &s, int kvh, int rt) {
     const int tok0 = sh.token0(rt), hg = sh.hpt == 1 ? 0 : rt % sh.hpt;
@@ -227,7 +242,7 @@ struct PagedUnit {
     head0 = kvh * sh.G + hg * sh.rows;
     heads = min(sh.gw, sh.G - hg * sh.rows);
     gw = sh.gw;
-    last0 = (int64_t)s.len - s.qlen + tok0;
+    last0 = s.len - s.qlen + tok0;
     sh.keys(s, rt, k0, k1);
   }
   // Packed row and query head of row r; false: the unit has no such row.
@@ -253,9 +268,9 @@ struct PagedPart {
       ++wk.w;
       return;
     }
-    const int64_t ue = wk.us + n, end = wk.w_end < ue ? wk.w_end : ue;
-    t0 = first + (int)(wk.w - wk.us);
-    t1 = first + (int)(end - wk.us);
+    const int ue = wk.us + n, end = min(wk.w_end, ue);
+    t0 = first + wk.w - wk.us;
+    t1 = first + end - wk.us;
     const bool begins = wk.w == wk.us, ends = end == ue;
     partial = begins && ends ? -1 : begins ? 2 * wk.id + 1 : 2 * wk.id;
     wk.w = end;
@@ -330,7 +345,8 @@ paged_rows_kernel(PagedAttnParams p) {
     uint4 qx[ST];
 #pragma unroll
     for (int st = 0; st < ST; ++st) qx[st] = load16(qp + 64 * st);
-    const int64_t last = u.last0 + (own ? qt - u.row0 : 0), from = p.sh.window > 0 ? last - p.sh.window : -1;
+    const int last = u.last0 + (own ? qt - u.row0 : 0);
+    const int from = p.sh.window > 0 && last >= p.sh.window ? last - p.sh.window : -1;
     const int32_t *table = p.table + wk.b * p.table_stride;
     const char *kb = p.k + wk.kvh * p.head_b, *vb = p.v + wk.kvh * p.head_b;
 
@@ -414,7 +430,7 @@ paged_rows_kernel(PagedAttnParams p) {
       // Scores in base 2; keys that the row does not see are -inf.
       const int key0 = key_of(t, 0) - col;
       const bool edge = u.tokens > 1 && (key0 + 31 > u.last0 ||
-                                         (p.sh.window > 0 && key0 <= u.last0 + u.tokens - 1 - p.sh.window));
+                                         (p.sh.window > 0 && key0 + p.sh.window <= u.last0 + u.tokens - 1));
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
@@ -676,12 +692,13 @@ __global__ void __launch_bounds__(kPgThreads, KT <= 4 ? 2 : 1) paged_chunk_kerne
 
     // Hidden keys' scores of tile t become -inf.
     auto hide = [&](f32x16_t(&s)[RG][2], int t, uint64_t there) {
-      const int64_t key0 = (int64_t)t << kChunkTileShift;
-      const bool edge = key0 + 63 > u.last0 + tok_a || (p.sh.window > 0 && key0 <= u.last0 + tok_z - p.sh.window);
+      const int key0 = t << kChunkTileShift;
+      const bool edge = key0 + 63 > u.last0 + tok_a || (p.sh.window > 0 && key0 + p.sh.window <= u.last0 + tok_z);
       if (!edge && there == ~uint64_t(0)) return;
 #pragma unroll
       for (int g = 0; g < RG; ++g) {
-        const int64_t hi = u.last0 + tok[g] + 1 - key0, lo = p.sh.window > 0 ? hi - p.sh.window : 0;
+        // Keys [lo, hi) of the tile; a window as long as the keys hides none.
+        const int hi = u.last0 + tok[g] + 1 - key0, lo = p.sh.window > 0 && hi > 0 ? hi - p.sh.window : 0;
         uint64_t v = hi >= 64 ? ~uint64_t(0) : hi <= 0 ? 0 : (uint64_t(1) << hi) - 1;
         if (lo > 0) v &= lo >= 64 ? 0 : ~uint64_t(0) << lo;
         v = (v & there) >> (4 * hf);
@@ -967,8 +984,13 @@ __global__ void __launch_bounds__(kPgThreads) paged_combine_kernel(PagedAttnPara
 }
 
 // ------------------------------------------------------------------- host
+// Units of at most this many tiles (by the host's bound of the keys) are never
+// divided: one launch, no partial rows.
+constexpr int kWholeTiles = 4;
+
 struct PagedPlan {
   PagedShape sh;
+  int64_t weight;  // a bound of the call's weights
   int blocks, least;
   bool chunk;  // the chunk kernel
   bool split;  // units are cut into many parts
@@ -992,15 +1014,25 @@ static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
   w.chunk = c.dtype != KIV_DTYPE_F32 && (int64_t)std::min(b.max_q_len, b.total_q) * G > kRowsOfUnit &&
             c.page_size % chunk_load_rows(c.head_dim) == 0 && c.stride[2] >= 0 && c.stride[2] < (1 << 24);
   const int rows = w.chunk ? chunk_rows(c.head_dim) : kRowsOfUnit, shift = w.chunk ? kChunkTileShift : kRowsTileShift;
-  w.sh = PagedShape::of(b.total_q, c.num_kv_heads, G, rows, cap, shift, a.window, false);
+  const int window = std::min(a.window, 1 << 30);  // no table is as long
+  w.sh = PagedShape::of(b.total_q, c.num_kv_heads, G, rows, cap, shift, window, false);
   // More than the call's units and tiles, by what the host knows of them.
   const int64_t units =
       ((int64_t)b.total_q / w.sh.tpu + std::min(b.num_seqs, b.total_q)) * w.sh.hpt * c.num_kv_heads;
-  const int64_t keys = a.window > 0 ? std::min<int64_t>(most_keys, (int64_t)a.window + w.sh.tpu) : most_keys;
-  const int64_t tiles = (keys >> shift) + 2;
-  w.least = 1;
+  w.weight = units * ((cap >> shift) + 2);
+  const int64_t keys = window > 0 ? std::min<int64_t>(most_keys, (int64_t)window + w.sh.tpu) : most_keys;
+  const int64_t tiles = (keys >> shift) + 1;
   const int slots = device_cu_count() * (w.chunk && c.head_dim > 128 ? 1 : 2);
-  w.blocks = (int)std::max<int64_t>(8, std::min<int64_t>(slots, units * tiles) & ~int64_t(7));
+  w.least = 1;
+  w.split = false;
+  w.cuts_x = w.cuts_y = 0;
+  w.m_off = w.l_off = w.o_off = w.total = 0;
+  if (tiles <= kWholeTiles) {
+    w.sh.whole = 1;
+    w.blocks = (int)std::min<int64_t>(4 * slots, units);
+    return w;
+  }
+  w.blocks = (int)std::max<int64_t>(8, std::min<int64_t>(slots, units * (tiles + 1)) & ~int64_t(7));
   w.split = w.blocks > 6 * units;
   w.cuts_x = (int)std::min<int64_t>(w.blocks, std::max<int64_t>(1, units));
   const int most_rows = (int)std::min<int64_t>(rows, (int64_t)w.sh.gw * std::max(1, std::min(w.sh.tpu, b.max_q_len)));
@@ -1026,6 +1058,8 @@ static int paged_attention_check(const kiv_paged_attention_args_t *a, const char
   if (a->num_q_heads < 1 || a->num_q_heads % c.num_kv_heads)
     return fail(KIV_ERR_INVALID, "%s: bad head geometry", who);
   if (a->window < 0) return fail(KIV_ERR_INVALID, "%s: negative window", who);
+  if ((int64_t)a->batch.table_width * c.page_size > (1 << 30))
+    return fail(KIV_ERR_UNSUPPORTED, "%s: the block table spans over 2^30 keys", who);
   // Hidden scores are -inf behind the scale, and the maximum is taken there.
   if (!(a->scaling > 0.f) || !(a->scaling < INFINITY))
     return fail(KIV_ERR_UNSUPPORTED, "%s: scaling must be positive and finite", who);
@@ -1068,7 +1102,9 @@ int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream
   if ((((uintptr_t)a->q | (uintptr_t)a->out) & 15) || a->q_stride[0] % vec || a->q_stride[1] % vec)
     return fail(KIV_ERR_INVALID, "%s: rows must be 16-byte aligned", who);
   const PagedPlan w = paged_plan(*a);
-  if (!a->workspace || a->workspace_bytes < w.total || ((uintptr_t)a->workspace & 255))
+  if (w.weight > 2000000000)
+    return fail(KIV_ERR_UNSUPPORTED, "%s: too much work for one call (%lld tiles)", who, (long long)w.weight);
+  if (w.total > 0 && (!a->workspace || a->workspace_bytes < w.total || ((uintptr_t)a->workspace & 255)))
     return fail(KIV_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes "
                 "(kiv_paged_attention_workspace_size)", who, w.total);
   PagedAttnParams p;
@@ -1095,7 +1131,7 @@ int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream
   p.scale_log2 = a->scaling * kPgLog2e;
   p.out = (char *)a->out;
   char *ws = (char *)a->workspace;
-  p.cuts = (PagedCut *)ws;
+  p.cuts = w.total > 0 ? (PagedCut *)ws : nullptr;
   p.ws_m = (float *)(ws + w.m_off);
   p.ws_l = (float *)(ws + w.l_off);
   p.ws_o = (float *)(ws + w.o_off);
@@ -1111,6 +1147,7 @@ int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream
           hipLaunchKernelGGL((paged_chunk_kernel<DTV, DV / 32, chunk_groups(DV)>), grid, dim3(kPgThreads), 0, st, p);
       }
       if (!w.chunk) hipLaunchKernelGGL((paged_rows_kernel<DTV, DV>), grid, dim3(kPgThreads), 0, st, p);
+      if (w.total == 0) return;
       if (w.split) hipLaunchKernelGGL((paged_combine_kernel<DTV, true>), cgrid, dim3(kPgThreads), 0, st, p, D);
       else hipLaunchKernelGGL((paged_combine_kernel<DTV, false>), cgrid, dim3(kPgThreads), 0, st, p, D);
     };

@@ -77,11 +77,10 @@ struct PagedShape {
   KIV_HD int tokens(const PagedSeq &s, int tok0) const { return s.qlen - tok0 < tpu ? s.qlen - tok0 : tpu; }
   // Keys [k0, k1) that some row of unit rt sees.
   KIV_HD void keys(const PagedSeq &s, int rt, int &k0, int &k1) const {
-    const int tok0 = token0(rt);
-    const int64_t off = (int64_t)s.len - s.qlen, last = off + tok0 + tokens(s, tok0);
-    const int64_t first = window > 0 ? off + tok0 - window + 1 : 0;
-    k1 = (int)(last < 0 ? 0 : last < cap ? last : cap);
-    k0 = (int)(first < 0 ? 0 : first < k1 ? first : k1);
+    const int tok0 = token0(rt), from = s.len - s.qlen + tok0;  // the first token's key
+    const int last = from + tokens(s, tok0);
+    k1 = last < 0 ? 0 : last < cap ? last : cap;
+    k0 = window > 0 && from >= window ? from - window + 1 : 0;
     if (k0 >= k1) k0 = k1 = 0;
   }
   // First tile and number of tiles of the keys [k0, k1); a unit that sees no
@@ -99,17 +98,23 @@ struct PagedShape {
 // The weights 0 .. total - 1 in n shares, equal to within one: block i takes
 // [start(i), start(i + 1)).
 struct PagedShares {
-  int64_t total;
-  int n;
-  // Blocks that share the work: none gets less than `least`, a multiple of
-  // the eight dies where there are that many.
-  KIV_HD static int blocks(int64_t total, int most, int least) {
-    const int64_t n = total / least;
-    const int m = (int)(n < most ? n : most);
-    return m >= 8 ? m & ~7 : m > 0 ? m : 1;
+  int total, n, per, rem;
+  // Dealt to at most `most` blocks, none with less than `least`; many blocks
+  // are a multiple of the eight dies.
+  KIV_HD static PagedShares deal(int total, int most, int least) {
+    PagedShares s;
+    const int want = total / least, m = want < most ? want : most;
+    s.total = total;
+    s.n = m >= 64 ? m & ~7 : m > 0 ? m : 1;
+    s.per = total / s.n;
+    s.rem = total - s.per * s.n;
+    return s;
   }
-  KIV_HD int64_t start(int i) const { return total * i / n; }
-  KIV_HD int block_of(int64_t w) const { return (int)(((w + 1) * n - 1) / total); }
+  KIV_HD int start(int i) const { return i * per + (i < rem ? i : rem); }
+  KIV_HD int block_of(int w) const {
+    const int longer = rem * (per + 1);  // weights of the shares that are one longer
+    return w < longer ? w / (per + 1) : rem + (w - longer) / per;
+  }
 };
 
 }  // namespace kiv

@@ -64,8 +64,9 @@ class PagedKVCache:
         self.k, self.v = k, v
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype, self.device = k.dtype, k.device
-        self._args = nat.PagedCacheArgs(k.data_ptr(), v.data_ptr(), nat.strides(k, 3), self.num_pages, self.page_size,
-                                        self.num_kv_heads, self.head_dim, nat.dtype_code(k.dtype), 0)
+        self._args = nat.PagedCacheArgs(k.data_ptr(), v.data_ptr(), nat.layout(k).strides, self.num_pages,
+                                        self.page_size, self.num_kv_heads, self.head_dim, nat.dtype_code(k.dtype), 0)
+        self._geometry = (self.num_kv_heads, self.head_dim, self.page_size, k.dtype, k.stride(2))
 
     def memory_bytes(self) -> int:
         """Bytes of the pool's K and V rows."""
@@ -115,11 +116,14 @@ class PagedBatch:
         self._args = nat.PagedBatchArgs(
             cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0) if S > 1 else 0, S, W, 0,
             big if max_q_len is None else min(max_q_len, big), big if max_kv_len is None else min(max_kv_len, big), 0)
+        self._geometry = (S, W, self._args.max_q_len, self._args.max_kv_len, self.device)
 
 
-def _packed(t: torch.Tensor, name: str, cache: PagedKVCache, batch: PagedBatch, heads: int | None) -> torch.Tensor:
-    if t.dim() != 3 or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {cache.head_dim}], got {tuple(t.shape)}")
+def _packed(t: torch.Tensor, name: str, cache: PagedKVCache, batch: PagedBatch, heads: int | None):
+    """(tensor, address, layout) of packed rows [tokens, heads, head_dim]."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {cache.head_dim}], got {tuple(shape)}")
     if t.dtype != cache.dtype:
         raise TypeError(f"{name} is {t.dtype}, the cache {cache.dtype}")
     if t.device != cache.device or batch.device != cache.device:
@@ -144,25 +148,29 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
     there is dropped.
     """
     no_grad_check("paged_append", q, k, v)
-    k = _packed(k, "k", cache, batch, cache.num_kv_heads)
-    v = _packed(v, "v", cache, batch, cache.num_kv_heads)
+    args = nat.PagedAppendArgs()
+    args.cache, args.batch = cache._args, batch._args
+    ksrc, args.k, lay = _packed(k, "k", cache, batch, cache.num_kv_heads)
+    args.k_stride = lay.strides
+    vsrc, args.v, lay = _packed(v, "v", cache, batch, cache.num_kv_heads)
+    args.v_stride = lay.strides
     T = k.shape[0]
     if v.shape[0] != T:
         raise ValueError(f"k has {T} tokens, v {v.shape[0]}")
     dev, D = cache.device, cache.head_dim
-    args = nat.PagedAppendArgs()
-    args.cache, args.batch = cache._args, batch._args
     args.batch.total_q = T
-    args.k, args.k_stride = k.data_ptr(), nat.strides(k, 2)
-    args.v, args.v_stride = v.data_ptr(), nat.strides(v, 2)
     if q is not None:
-        src = _packed(q, "q", cache, batch, None)
-        if src.shape[0] != T:
-            raise ValueError(f"k has {T} tokens, q {src.shape[0]}")
-        q_out = torch.empty_like(src) if q_out is None else out_rows(q_out, q, "q_out")
+        src, args.q, lay = _packed(q, "q", cache, batch, None)
+        args.q_stride = lay.strides
+        if q.shape[0] != T:
+            raise ValueError(f"k has {T} tokens, q {q.shape[0]}")
         args.num_q_heads = q.shape[1]
-        args.q, args.q_stride = src.data_ptr(), nat.strides(src, 2)
-        args.q_out, args.q_out_stride = q_out.data_ptr(), nat.strides(q_out, 2)
+        if q_out is None:
+            q_out = torch.empty_like(src)
+            args.q_out, args.q_out_stride = q_out.data_ptr(), nat.layout(q_out).strides
+        else:
+            args.q_out, lay = out_rows(q_out, q, "q_out")
+            args.q_out_stride = lay.strides
         if q_norm is not None:
             args.q_norm = q_norm.check(D, dev)
     elif q_norm is not None or q_out is not None:
@@ -173,7 +181,7 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
         args.v_norm = v_norm.check(D, dev)
     if rotary is not None:
         args.rotary = rotary._args
-        rotary.fill(args.rotary, positions, 1, T, dev, batched=False)
+        rotary.fill(args.rotary, positions, 1, T, dev, False)
     elif positions is not None:
         raise ValueError("positions need a rotation")
     nat.call("kiv_paged_append", args, dev)
@@ -193,29 +201,36 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
     new tensor: undefined).
     """
     no_grad_check("paged_attention", query)
-    q = _packed(query, "query", cache, batch, None)
-    T, hq, D = q.shape
-    if out is None:
-        out = torch.empty((T, hq, D), dtype=q.dtype, device=q.device)
-    elif out_rows(out, query, "out") is not None and not out.is_contiguous():
-        raise ValueError("out must be contiguous")
-    if window < 0:
-        raise ValueError(f"window must not be negative, got {window}")
     args = nat.PagedAttentionArgs()
     args.cache, args.batch = cache._args, batch._args
+    q, args.q, lay = _packed(query, "query", cache, batch, None)
+    args.q_stride = lay.strides
+    T, hq, D = query.shape
+    dev = cache.device
+    if out is None:
+        out = torch.empty((T, hq, D), dtype=q.dtype, device=dev)
+    else:
+        out_rows(out, query, "out")
+        if not out.is_contiguous():
+            raise ValueError("out must be contiguous")
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
     args.batch.total_q = T
-    args.q, args.q_stride = q.data_ptr(), nat.strides(q, 2)
     args.out = out.data_ptr()
     args.num_q_heads, args.window, args.scaling = hq, min(window, 2**31 - 1), scaling
-    ws = _workspace(args, cache.device)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
-    nat.call("kiv_paged_attention", args, cache.device)
+    # Scratch of this call, from torch's allocator on the current stream: calls
+    # on other streams, and captured graphs, have their own.
+    key = (T, hq, window, cache._geometry, batch._geometry)
+    need = _ws_sizes.get(key)
+    if need is None:
+        with torch.cuda.device(dev):
+            need = nat.lib().kiv_paged_attention_workspace_size(args)
+        if need and len(_ws_sizes) < 4096:
+            _ws_sizes[key] = need
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    nat.call("kiv_paged_attention", args, dev)
     return out
 
 
-def _workspace(args: nat.PagedAttentionArgs, device: torch.device) -> torch.Tensor:
-    """Scratch of one call, from torch's allocator on the current stream: calls
-    on other streams, and captured graphs, have their own."""
-    with torch.cuda.device(device):
-        need = nat.lib().kiv_paged_attention_workspace_size(args)
-    return torch.empty(need, dtype=torch.uint8, device=device)
+_ws_sizes: dict[tuple, int] = {}

@@ -37,12 +37,13 @@ class HeadNorm:
             raise ValueError(f"norm epsilon must not be negative, got {eps}")
         self.weight = weight
         self.eps = eps
+        self._at = None if weight is None else (weight.shape[0], weight.device)
         self._args = nat.HeadNormArgs(nat.ptr(weight), eps, 1)
 
     def check(self, head_dim: int, device: torch.device) -> nat.HeadNormArgs:
-        w = self.weight
-        if w is not None and (w.shape[0] != head_dim or w.device != device):
-            raise ValueError(f"norm weight is [{w.shape[0]}] on {w.device}, rows have head_dim {head_dim} on {device}")
+        at = self._at
+        if at is not None and at != (head_dim, device):
+            raise ValueError(f"norm weight is [{at[0]}] on {at[1]}, rows have head_dim {head_dim} on {device}")
         return self._args
 
 
@@ -79,68 +80,80 @@ class Rotary:
         self.interleaved = bool(interleaved)
         self.scale = float(scale)
         self.rot_dim = 2 * inv_freq.shape[0]
+        self.device = inv_freq.device
         self._args = nat.RotaryArgs(self.inv_freq.data_ptr(), nat.ptr(axes), None, nat._I64x3(), 0, 1, self.rot_dim,
                                     int(self.interleaved), self.scale, 0)
 
     def fill(self, dst: nat.RotaryArgs, positions: torch.Tensor | None, batch: int, tokens: int,
-             device: torch.device, batched: bool) -> torch.Tensor | None:
-        """Set the rotation in ``dst`` for positions [tokens], [batch, tokens]
-        (``batched``) or either behind an axis dimension; returns the tensor
-        the launch reads."""
-        if self.inv_freq.device != device:
-            raise ValueError(f"inv_freq is on {self.inv_freq.device}, rows on {device}")
+             device: torch.device, batched: bool) -> None:
+        """Set the positions in ``dst``: [tokens], [batch, tokens] (``batched``)
+        or either behind an axis dimension."""
+        if self.device != device:
+            raise ValueError(f"inv_freq is on {self.device}, rows on {device}")
+        lead = self.axes is not None
         if positions is None:
-            if self.axes is not None:
+            if lead:
                 raise ValueError("a rotation with several axes needs positions")
-            return None
-        if positions.dtype not in (torch.int64, torch.int32):
-            raise TypeError(f"positions must be int32 or int64, not {positions.dtype}")
+            return
         if positions.device != device:
             raise ValueError(f"positions are on {positions.device}, rows on {device}")
-        shape, st = positions.shape, positions.stride()
-        lead = 0 if self.axes is None else 1
-        if lead:
-            if len(shape) < 2 or shape[0] < 1:
-                raise ValueError("positions of a rotation with several axes need a leading axis dimension")
-            dst.num_axes = shape[0]
-            dst.position_stride[0] = st[0]
-        rest = shape[lead:]
-        if rest == (tokens,):
-            sb, stt = 0, st[lead]
-        elif batched and len(rest) == 2 and rest[0] in (1, batch) and rest[1] == tokens:
-            sb, stt = (0 if rest[0] == 1 else st[lead]), st[lead + 1]
-        else:
-            raise ValueError(f"positions {tuple(shape)} do not fit {batch} x {tokens} tokens")
-        dst.position_stride[1], dst.position_stride[2] = sb, stt
+        key = (positions.shape, positions.stride(), positions.dtype, lead, batched, batch, tokens)
+        got = _position_layouts.get(key)
+        if got is None:
+            got = _position_layout(*key)
+            if len(_position_layouts) < 4096:
+                _position_layouts[key] = got
+        dst.position_stride, dst.position_bytes, dst.num_axes = got
         dst.positions = positions.data_ptr()
-        dst.position_bytes = positions.element_size()
-        return positions
+
+
+_position_layouts: dict[tuple, tuple] = {}
+
+
+def _position_layout(shape, st, dtype, lead: bool, batched: bool, batch: int, tokens: int) -> tuple:
+    """(strides over axis, batch and token; bytes; axes) of positions."""
+    if dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"positions must be int32 or int64, not {dtype}")
+    axes, sa, rest = 1, 0, tuple(shape)
+    if lead:
+        if len(rest) < 2 or rest[0] < 1:
+            raise ValueError("positions of a rotation with several axes need a leading axis dimension")
+        axes, sa, rest = rest[0], st[0], rest[1:]
+    if rest == (tokens,):
+        sb, stt = 0, st[lead]
+    elif batched and len(rest) == 2 and rest[0] in (1, batch) and rest[1] == tokens:
+        sb, stt = (0 if rest[0] == 1 else st[lead]), st[lead + 1]
+    else:
+        raise ValueError(f"positions {tuple(shape)} do not fit {batch} x {tokens} tokens")
+    return nat._I64x3(sa, sb, stt), 8 if dtype == torch.int64 else 4, axes
 
 
 def no_grad_check(what: str, *tensors: torch.Tensor | None) -> None:
     """These kernels have no backward pass: refuse to drop a gradient."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
 
 
-def aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the kernels can load its rows (unit stride over
-    head_dim, 16-byte aligned), else a copy."""
-    vec = 16 // t.element_size()
-    st = t.stride()
-    ok = st[-1] == 1 and t.data_ptr() % 16 == 0
-    for n, s in zip(t.shape[:-1], st[:-1]):
-        ok = ok and (n == 1 or s % vec == 0)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+def aligned_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, nat.Layout]:
+    """(tensor, address, layout) of t where the kernels can load its rows (unit
+    stride over head_dim, 16-byte aligned), else of a copy."""
+    lay, at = nat.layout(t), t.data_ptr()
+    if lay.chunked and at & 15 == 0:
+        return t, at, lay
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), nat.layout(t)
 
 
-def out_rows(out: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
-    """Check a caller's output tensor."""
+def out_rows(out: torch.Tensor, like: torch.Tensor, what: str) -> tuple[int, nat.Layout]:
+    """Check a caller's output tensor: its address and layout."""
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{what} must be {tuple(like.shape)} {like.dtype} on {like.device}")
-    if aligned_rows(out) is not out:
+    lay, at = nat.layout(out), out.data_ptr()
+    if not lay.chunked or at & 15:
         raise ValueError(f"{what} rows must be 16-byte aligned, with unit stride over head_dim")
-    return out
+    return at, lay
 
 
 def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor | None, rotary: Rotary | None,
@@ -158,36 +171,43 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor |
     no_grad_check("norm_rope", q, k)
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("q and k must be [B, H, T, D]")
-    if not q.is_cuda:
+    dev = q.device
+    if dev.type != "cuda":
         raise ValueError("norm_rope needs GPU tensors")
     B, hq, T, D = q.shape
-    if k is not None and ((k.shape[0], k.shape[2], k.shape[3]) != (B, T, D) or k.dtype != q.dtype
-                          or k.device != q.device):
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
-    if k is None and (k_norm is not None or k_out is not None):
-        raise ValueError("k_norm and k_out need k")
     args = nat.NormRopeArgs()
-    dev = q.device
     args.dtype = nat.dtype_code(q.dtype)
     args.batch, args.num_q_heads, args.tokens, args.head_dim = B, hq, T, D
-    src = aligned_rows(q)
-    q_out = torch.empty_like(src) if q_out is None else out_rows(q_out, q, "q_out")
-    args.q, args.q_stride = src.data_ptr(), nat.strides(src, 3)
-    args.q_out, args.q_out_stride = q_out.data_ptr(), nat.strides(q_out, 3)
+    src, args.q, lay = aligned_rows(q)
+    args.q_stride = lay.strides
+    if q_out is None:
+        q_out = torch.empty_like(src)
+        args.q_out, args.q_out_stride = q_out.data_ptr(), nat.layout(q_out).strides
+    else:
+        args.q_out, lay = out_rows(q_out, q, "q_out")
+        args.q_out_stride = lay.strides
     if q_norm is not None:
         args.q_norm = q_norm.check(D, dev)
     if k is not None:
-        ksrc = aligned_rows(k)
-        k_out = torch.empty_like(ksrc) if k_out is None else out_rows(k_out, k, "k_out")
-        args.num_kv_heads = k.shape[1]
-        args.k, args.k_stride = ksrc.data_ptr(), nat.strides(ksrc, 3)
-        args.k_out, args.k_out_stride = k_out.data_ptr(), nat.strides(k_out, 3)
+        Bk, args.num_kv_heads, Tk, Dk = k.shape
+        if Bk != B or Tk != T or Dk != D or k.dtype != q.dtype or k.device != dev:
+            raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
+        ksrc, args.k, lay = aligned_rows(k)
+        args.k_stride = lay.strides
+        if k_out is None:
+            k_out = torch.empty_like(ksrc)
+            args.k_out, args.k_out_stride = k_out.data_ptr(), nat.layout(k_out).strides
+        else:
+            args.k_out, lay = out_rows(k_out, k, "k_out")
+            args.k_out_stride = lay.strides
         if k_norm is not None:
             args.k_norm = k_norm.check(D, dev)
+    elif k_norm is not None or k_out is not None:
+        raise ValueError("k_norm and k_out need k")
     if rotary is not None:
         if positions is None:
             raise ValueError("a rotation needs positions")
         args.rotary = rotary._args
-        rotary.fill(args.rotary, positions, B, T, dev, batched=True)
+        rotary.fill(args.rotary, positions, B, T, dev, True)
     nat.call("kiv_norm_rope", args, dev)
     return q_out, k_out

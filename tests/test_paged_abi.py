@@ -140,6 +140,9 @@ def test_paged_append_refusals(code, over):
     assert b"kiv_paged_append" in lib.kiv_last_error()
 
 
+LONG = dict(batch__table_width=1000, batch__max_kv_len=8000)  # keys that several blocks share
+
+
 def attention_args(**over):
     a = nat.PagedAttentionArgs()
     fill_cache(a)
@@ -164,9 +167,11 @@ def attention_args(**over):
     (nat.ERR_UNSUPPORTED, dict(scaling=0.0)),
     (nat.ERR_UNSUPPORTED, dict(scaling=float("nan"))),
     (nat.ERR_UNSUPPORTED, dict(scaling=float("inf"))),
-    (nat.ERR_INVALID, dict(workspace=None)),
-    (nat.ERR_INVALID, dict(workspace=AT + 16)),
-    (nat.ERR_INVALID, dict(workspace_bytes=64)),
+    (nat.ERR_INVALID, dict(LONG, workspace=None)),
+    (nat.ERR_INVALID, dict(LONG, workspace=AT + 16)),
+    (nat.ERR_INVALID, dict(LONG, workspace_bytes=64)),
+    (nat.ERR_UNSUPPORTED, dict(batch__table_width=(1 << 27) + 1)),
+    (nat.ERR_UNSUPPORTED, dict(LONG, batch__table_width=1 << 27, batch__total_q=1 << 20)),
 ])
 def test_paged_attention_refusals(code, over):
     lib = nat.lib()
@@ -179,7 +184,8 @@ def test_paged_workspace_size():
     assert lib.kiv_paged_attention_workspace_size(None) == 0
     assert lib.kiv_paged_attention_workspace_size(C.byref(attention_args(cache__head_dim=48))) == 0
     assert lib.kiv_paged_attention_workspace_size(C.byref(attention_args(batch__total_q=0))) == 0
-    assert lib.kiv_paged_attention_workspace_size(C.byref(attention_args())) > 0
+    assert lib.kiv_paged_attention_workspace_size(C.byref(attention_args())) == 0  # few keys: never divided
+    assert lib.kiv_paged_attention_workspace_size(C.byref(attention_args(**LONG))) > 0
     assert lib.kiv_paged_attention(C.byref(attention_args(batch__total_q=0, workspace=None)), None) == 0
     assert lib.kiv_paged_attention(None, None) == nat.ERR_INVALID
 

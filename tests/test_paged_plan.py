@@ -91,9 +91,7 @@ static void walk(int seed) {
   }
   if (total == 0) return;
   const int most = 8 * pick(1, 70), least = pick(1, 4);
-  PagedShares shares;
-  shares.total = total;
-  shares.n = PagedShares::blocks(total, most, least);
+  const PagedShares shares = PagedShares::deal((int)total, most, least);
   EXPECT(shares.n >= 1 && shares.n <= most && shares.n <= total);
   EXPECT(shares.start(0) == 0 && shares.start(shares.n) == total);
   std::map<int, int> written;              // partial slot -> unit
