@@ -66,7 +66,7 @@ class PagedKVCache:
         self.dtype, self.device = k.dtype, k.device
         self._args = nat.PagedCacheArgs(k.data_ptr(), v.data_ptr(), nat.layout(k).strides, self.num_pages,
                                         self.page_size, self.num_kv_heads, self.head_dim, nat.dtype_code(k.dtype), 0)
-        self._geometry = (self.num_kv_heads, self.head_dim, self.page_size, k.dtype, k.stride(2))
+        self._geometry = (tuple(k.shape), k.stride(), k.dtype)
 
     def memory_bytes(self) -> int:
         """Bytes of the pool's K and V rows."""
@@ -119,16 +119,14 @@ class PagedBatch:
         self._geometry = (S, W, self._args.max_q_len, self._args.max_kv_len, self.device)
 
 
-def _packed(t: torch.Tensor, name: str, cache: PagedKVCache, batch: PagedBatch, heads: int | None):
-    """(tensor, address, layout) of packed rows [tokens, heads, head_dim]."""
+def _packed_layout(t: torch.Tensor, name: str, cache: PagedKVCache, heads: int | None) -> nat.Layout:
+    """Layout of packed rows [tokens, heads, head_dim] that go with the cache."""
     shape = t.shape
     if len(shape) != 3 or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
         raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {cache.head_dim}], got {tuple(shape)}")
     if t.dtype != cache.dtype:
         raise TypeError(f"{name} is {t.dtype}, the cache {cache.dtype}")
-    if t.device != cache.device or batch.device != cache.device:
-        raise ValueError(f"{name} is on {t.device}, the batch on {batch.device}, the cache on {cache.device}")
-    return aligned_rows(t)
+    return nat.layout(t)
 
 
 def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor,
@@ -148,26 +146,37 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
     there is dropped.
     """
     no_grad_check("paged_append", q, k, v)
-    args = nat.PagedAppendArgs()
-    args.cache, args.batch = cache._args, batch._args
-    ksrc, args.k, lay = _packed(k, "k", cache, batch, cache.num_kv_heads)
-    args.k_stride = lay.strides
-    vsrc, args.v, lay = _packed(v, "v", cache, batch, cache.num_kv_heads)
-    args.v_stride = lay.strides
-    T = k.shape[0]
-    if v.shape[0] != T:
-        raise ValueError(f"k has {T} tokens, v {v.shape[0]}")
+    key = (cache._geometry, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype,
+           None if q is None else (q.shape, q.stride(), q.dtype))
+    plan = _append_plans.get(key)
+    if plan is None:
+        plan = _append_plan(cache, k, v, q)
+        if len(_append_plans) < 4096:
+            _append_plans[key] = plan
+    template, T, copy = plan
     dev, D = cache.device, cache.head_dim
+    if k.device != dev or v.device != dev or batch.device != dev or (q is not None and q.device != dev):
+        raise ValueError(f"k, v, q, the batch and the cache must be on one device ({dev})")
+    args = nat.PagedAppendArgs.from_buffer_copy(template)
+    args.cache, args.batch = cache._args, batch._args
     args.batch.total_q = T
+    at, vat = k.data_ptr(), v.data_ptr()
+    if copy or (at | vat) & 15:
+        k, at, lay = aligned_rows(k)
+        args.k_stride = lay.strides
+        v, vat, lay = aligned_rows(v)
+        args.v_stride = lay.strides
+    args.k, args.v = at, vat
     if q is not None:
-        src, args.q, lay = _packed(q, "q", cache, batch, None)
-        args.q_stride = lay.strides
-        if q.shape[0] != T:
-            raise ValueError(f"k has {T} tokens, q {q.shape[0]}")
-        args.num_q_heads = q.shape[1]
+        at = q.data_ptr()
+        if copy or at & 15:
+            q, at, lay = aligned_rows(q)
+            args.q_stride = lay.strides
+            args.q_out_stride = nat.layout(torch.empty_like(q, device="meta")).strides
+        args.q = at
         if q_out is None:
-            q_out = torch.empty_like(src)
-            args.q_out, args.q_out_stride = q_out.data_ptr(), nat.layout(q_out).strides
+            q_out = torch.empty_like(q)
+            args.q_out = q_out.data_ptr()
         else:
             args.q_out, lay = out_rows(q_out, q, "q_out")
             args.q_out_stride = lay.strides
@@ -188,6 +197,28 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
     return q_out
 
 
+_append_plans: dict[tuple, tuple] = {}
+
+
+def _append_plan(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None) -> tuple:
+    """What a call's shapes, strides and dtypes give: (its arguments without
+    addresses, tokens, whether rows must be copied)."""
+    args = nat.PagedAppendArgs()
+    kl, vl = _packed_layout(k, "k", cache, cache.num_kv_heads), _packed_layout(v, "v", cache, cache.num_kv_heads)
+    args.k_stride, args.v_stride = kl.strides, vl.strides
+    T, copy = k.shape[0], not (kl.chunked and vl.chunked)
+    if v.shape[0] != T:
+        raise ValueError(f"k has {T} tokens, v {v.shape[0]}")
+    if q is not None:
+        ql = _packed_layout(q, "q", cache, None)
+        if q.shape[0] != T:
+            raise ValueError(f"k has {T} tokens, q {q.shape[0]}")
+        args.num_q_heads, args.q_stride = q.shape[1], ql.strides
+        args.q_out_stride = nat.layout(torch.empty_like(q, device="meta")).strides
+        copy = copy or not ql.chunked
+    return args, T, copy
+
+
 def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, scaling: float, window: int = 0,
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(q K^T * scaling) V of the batch's packed rows [tokens, Hq, D]
@@ -201,36 +232,53 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
     new tensor: undefined).
     """
     no_grad_check("paged_attention", query)
-    args = nat.PagedAttentionArgs()
-    args.cache, args.batch = cache._args, batch._args
-    q, args.q, lay = _packed(query, "query", cache, batch, None)
-    args.q_stride = lay.strides
-    T, hq, D = query.shape
     dev = cache.device
+    if query.device != dev or batch.device != dev:
+        raise ValueError(f"query is on {query.device}, the batch on {batch.device}, the cache on {dev}")
+    key = (query.shape, query.stride(), query.dtype, window, cache._geometry, batch._geometry)
+    plan = _attention_plans.get(key)
+    if plan is None:
+        plan = _attention_plan(query, cache, batch, window)
+        if len(_attention_plans) < 4096:
+            _attention_plans[key] = plan
+    template, need, T, copy = plan
+    args = nat.PagedAttentionArgs.from_buffer_copy(template)
+    args.cache, args.batch = cache._args, batch._args
+    args.batch.total_q = T
+    q, at = query, query.data_ptr()
+    if copy or at & 15:
+        q, at, lay = aligned_rows(query)
+        args.q_stride = lay.strides
     if out is None:
-        out = torch.empty((T, hq, D), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=dev)
     else:
         out_rows(out, query, "out")
         if not out.is_contiguous():
             raise ValueError("out must be contiguous")
-    if window < 0:
-        raise ValueError(f"window must not be negative, got {window}")
-    args.batch.total_q = T
-    args.out = out.data_ptr()
-    args.num_q_heads, args.window, args.scaling = hq, min(window, 2**31 - 1), scaling
-    # Scratch of this call, from torch's allocator on the current stream: calls
-    # on other streams, and captured graphs, have their own.
-    key = (T, hq, window, cache._geometry, batch._geometry)
-    need = _ws_sizes.get(key)
-    if need is None:
-        with torch.cuda.device(dev):
-            need = nat.lib().kiv_paged_attention_workspace_size(args)
-        if need and len(_ws_sizes) < 4096:
-            _ws_sizes[key] = need
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    args.q, args.out, args.scaling = at, out.data_ptr(), scaling
+    if need:
+        # Scratch of this call, from torch's allocator on the current stream:
+        # calls on other streams, and captured graphs, have their own.
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
     nat.call("kiv_paged_attention", args, dev)
     return out
 
 
-_ws_sizes: dict[tuple, int] = {}
+_attention_plans: dict[tuple, tuple] = {}
+
+
+def _attention_plan(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, window: int) -> tuple:
+    """What a call's shapes, strides, dtypes and bounds give: (its arguments
+    without addresses, workspace bytes, tokens, whether the query must be
+    copied)."""
+    lay = _packed_layout(query, "query", cache, None)
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    args = nat.PagedAttentionArgs()
+    args.cache, args.batch = cache._args, batch._args
+    args.batch.total_q, args.num_q_heads = query.shape[0], query.shape[1]
+    args.q_stride, args.window, args.scaling = lay.strides, min(window, 2**31 - 1), 1.0
+    with torch.cuda.device(cache.device):
+        need = nat.lib().kiv_paged_attention_workspace_size(args)
+    return args, need, query.shape[0], not lay.chunked

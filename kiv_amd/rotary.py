@@ -169,34 +169,41 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor |
     rotated width of 32 bytes.  Returns (q_out, k_out).
     """
     no_grad_check("norm_rope", q, k)
-    if q.dim() != 4 or (k is not None and k.dim() != 4):
-        raise ValueError("q and k must be [B, H, T, D]")
     dev = q.device
     if dev.type != "cuda":
         raise ValueError("norm_rope needs GPU tensors")
-    B, hq, T, D = q.shape
-    args = nat.NormRopeArgs()
-    args.dtype = nat.dtype_code(q.dtype)
-    args.batch, args.num_q_heads, args.tokens, args.head_dim = B, hq, T, D
-    src, args.q, lay = aligned_rows(q)
-    args.q_stride = lay.strides
+    key = (q.shape, q.stride(), q.dtype, None if k is None else (k.shape, k.stride(), k.dtype))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _plan(q, k)
+        if len(_plans) < 4096:
+            _plans[key] = plan
+    template, B, T, D, copy_q, copy_k = plan
+    args = nat.NormRopeArgs.from_buffer_copy(template)
+    at = q.data_ptr()
+    if copy_q or at & 15:
+        q, at, lay = aligned_rows(q)
+        args.q_stride = args.q_out_stride = lay.strides
+    args.q = at
     if q_out is None:
-        q_out = torch.empty_like(src)
-        args.q_out, args.q_out_stride = q_out.data_ptr(), nat.layout(q_out).strides
+        q_out = torch.empty_like(q)
+        args.q_out = q_out.data_ptr()
     else:
         args.q_out, lay = out_rows(q_out, q, "q_out")
         args.q_out_stride = lay.strides
     if q_norm is not None:
         args.q_norm = q_norm.check(D, dev)
     if k is not None:
-        Bk, args.num_kv_heads, Tk, Dk = k.shape
-        if Bk != B or Tk != T or Dk != D or k.dtype != q.dtype or k.device != dev:
-            raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
-        ksrc, args.k, lay = aligned_rows(k)
-        args.k_stride = lay.strides
+        if k.device != dev:
+            raise ValueError(f"k is on {k.device}, q on {dev}")
+        at = k.data_ptr()
+        if copy_k or at & 15:
+            k, at, lay = aligned_rows(k)
+            args.k_stride = args.k_out_stride = lay.strides
+        args.k = at
         if k_out is None:
-            k_out = torch.empty_like(ksrc)
-            args.k_out, args.k_out_stride = k_out.data_ptr(), nat.layout(k_out).strides
+            k_out = torch.empty_like(k)
+            args.k_out = k_out.data_ptr()
         else:
             args.k_out, lay = out_rows(k_out, k, "k_out")
             args.k_out_stride = lay.strides
@@ -211,3 +218,25 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor |
         rotary.fill(args.rotary, positions, B, T, dev, True)
     nat.call("kiv_norm_rope", args, dev)
     return q_out, k_out
+
+
+_plans: dict[tuple, tuple] = {}
+
+
+def _plan(q: torch.Tensor, k: torch.Tensor | None) -> tuple:
+    """What a call's shapes, strides and dtypes give: (its arguments without
+    addresses, B, T, D, q must be copied, k must be copied)."""
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("q and k must be [B, H, T, D]")
+    B, hq, T, D = q.shape
+    if k is not None and ((k.shape[0], k.shape[2], k.shape[3]) != (B, T, D) or k.dtype != q.dtype):
+        raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
+    args = nat.NormRopeArgs(batch=B, tokens=T, num_q_heads=hq, head_dim=D, dtype=nat.dtype_code(q.dtype))
+    # The memory order torch gives new tensors like these.
+    lay, args.q_out_stride = nat.layout(q), nat.layout(torch.empty_like(q, device="meta")).strides
+    args.q_stride = lay.strides
+    if k is None:
+        return args, B, T, D, not lay.chunked, False
+    klay, args.k_out_stride = nat.layout(k), nat.layout(torch.empty_like(k, device="meta")).strides
+    args.num_kv_heads, args.k_stride = k.shape[1], klay.strides
+    return args, B, T, D, not lay.chunked, not klay.chunked
