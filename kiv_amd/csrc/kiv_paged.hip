@@ -58,7 +58,7 @@ struct PagedAttnParams {
   int seqs, num_pages, page_size, hq;
   FastDiv page_div;
   PagedShape sh;
-  int blocks, least;  // most blocks that share the work, least tiles of a share
+  int blocks;  // most blocks that share the work
   float scale_log2;
   char *out;
   PagedCut *cuts;  // [blocks]
@@ -184,7 +184,7 @@ struct PagedWork {
   // order stays below by the host's check).
   __device__ __forceinline__ bool deal(const PagedAttnParams &p, int total, float ftotal) {
     if (total <= 0 || ftotal > 2.1e9f) return false;
-    shares = PagedShares::deal(total, p.blocks, p.least);
+    shares = PagedShares::deal(total, p.blocks);
     if ((int)blockIdx.x >= shares.n) return false;
     // Blocks are dealt to the eight dies in turn: a die takes neighbouring
     // shares, which read the same keys through its L2.
@@ -991,7 +991,7 @@ constexpr int kWholeTiles = 4;
 struct PagedPlan {
   PagedShape sh;
   int64_t weight;  // a bound of the call's weights
-  int blocks, least;
+  int blocks;
   bool chunk;  // the chunk kernel
   bool split;  // units are cut into many parts
   int cuts_x, cuts_y;  // the combine's grid
@@ -1022,8 +1022,11 @@ static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
   w.weight = units * ((cap >> shift) + 2);
   const int64_t keys = window > 0 ? std::min<int64_t>(most_keys, (int64_t)window + w.sh.tpu) : most_keys;
   const int64_t tiles = (keys >> shift) + 1;
-  const int slots = device_cu_count() * (w.chunk && c.head_dim > 128 ? 1 : 2);
-  w.least = 1;
+  // Blocks that a compute unit holds at once: two, or one where a row's
+  // operands take a whole wave's registers (32 sequences of up to 8192 keys of
+  // 256-wide heads dealt to twice as many 44 us, 37 by this).
+  const bool one = w.chunk ? c.head_dim > 128 : c.head_dim * elem_bytes(c.dtype) >= 512;
+  const int slots = device_cu_count() * (one ? 1 : 2);
   w.split = false;
   w.cuts_x = w.cuts_y = 0;
   w.m_off = w.l_off = w.o_off = w.total = 0;
@@ -1127,7 +1130,6 @@ int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream
   p.page_div = FastDiv::of(c.page_size);
   p.sh = w.sh;
   p.blocks = w.blocks;
-  p.least = w.least;
   p.scale_log2 = a->scaling * kPgLog2e;
   p.out = (char *)a->out;
   char *ws = (char *)a->workspace;

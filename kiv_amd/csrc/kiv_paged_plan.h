@@ -99,13 +99,13 @@ struct PagedShape {
 // [start(i), start(i + 1)).
 struct PagedShares {
   int total, n, per, rem;
-  // Dealt to at most `most` blocks, none with less than `least`; many blocks
-  // are a multiple of the eight dies.
-  KIV_HD static PagedShares deal(int total, int most, int least) {
+  // Dealt to at most `most` blocks, none without a weight; many blocks are a
+  // multiple of the eight dies.
+  KIV_HD static PagedShares deal(int total, int most) {
     PagedShares s;
-    const int want = total / least, m = want < most ? want : most;
+    const int m = total < most ? total : most;
     s.total = total;
-    s.n = m >= 64 ? m & ~7 : m > 0 ? m : 1;
+    s.n = m >= 64 ? m & ~7 : m;
     s.per = total / s.n;
     s.rem = total - s.per * s.n;
     return s;

@@ -90,8 +90,8 @@ static void walk(int seed) {
       }
   }
   if (total == 0) return;
-  const int most = 8 * pick(1, 70), least = pick(1, 4);
-  const PagedShares shares = PagedShares::deal((int)total, most, least);
+  const int most = pick(1, 560);
+  const PagedShares shares = PagedShares::deal((int)total, most);
   EXPECT(shares.n >= 1 && shares.n <= most && shares.n <= total);
   EXPECT(shares.start(0) == 0 && shares.start(shares.n) == total);
   std::map<int, int> written;              // partial slot -> unit
