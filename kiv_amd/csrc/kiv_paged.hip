@@ -537,13 +537,12 @@ paged_rows_kernel(PagedAttnParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Units of many rows (16-bit types): 4 waves of RG groups of 32 rows.
+// Units of 128 rows (16-bit types): 4 waves of 32.
 //
 // K and V tiles of 64 keys go from their pages straight to LDS, as rows,
 // double-buffered, their 16-byte chunks permuted so that operand reads spread
 // over the banks (K chunk c of row r at c ^ xk(r), V chunk c at c ^ 4 xv(r):
-// the loading lanes fetch the permuted chunk).  A wave reads each operand
-// once for its RG groups.
+// the loading lanes fetch the permuted chunk).
 //   S^T = K Q^T with 32x32 matrix instructions: lane l gives row l % 32 of a
 //   32-key sub-tile of K (A) and its own query row l % 32 (B, in registers
 //   for the whole unit), dims 16 st + 8 (l / 32) .. + 7 of step st, and
@@ -553,14 +552,13 @@ paged_rows_kernel(PagedAttnParams p) {
 // One iteration forms the scores of the next tile beside the exponentials of
 // this one, then adds this tile's values beside the next one's maxima, so
 // that vector and matrix instructions alternate in one wave's stream.
-template <int DT, int KT, int RG> struct ChunkGeom {
+template <int KT> struct ChunkGeom {
   static constexpr int D = 32 * KT, CPR = D / 8;
   static constexpr int CP = CPR <= 4 ? 4 : CPR <= 8 ? 8 : CPR <= 16 ? 16 : 32;  // chunks of an LDS row
   static constexpr int RPI = 64 / CP;   // rows of a load instruction
   static constexpr int NJ = CP / 4;     // load instructions of a wave for a tile of K (of V)
   static constexpr int TILE = 64 * CP * 16;  // LDS bytes of a tile
   static constexpr int KS = D / 16, ND = D / 32;
-  static constexpr int ROWS = 128 * RG;
   static __device__ __forceinline__ int xk(int r) { return CP >= 16 ? r & 15 : (r / (16 / CP)) & (CP - 1); }
   static __device__ __forceinline__ int xv(int r) { return CP >= 16 ? r & 3 : CP == 8 ? (r >> 1) & 1 : 0; }
 };
@@ -572,9 +570,9 @@ constexpr int kPgWaitAll = 0x0070;  // s_waitcnt vmcnt(0) lgkmcnt(0)
 // instructions that are to issue between matrix instructions.
 template <typename T> __device__ __forceinline__ void stay(T &x) { asm volatile("" : "+v"(x)); }
 
-template <int DT, int KT, int RG>
+template <int DT, int KT>
 __global__ void __launch_bounds__(kPgThreads, KT <= 4 ? 2 : 1) paged_chunk_kernel(PagedAttnParams p) {
-  using Geo = ChunkGeom<DT, KT, RG>;
+  using Geo = ChunkGeom<KT>;
   constexpr int D = Geo::D, CP = Geo::CP, CPR = Geo::CPR, RPI = Geo::RPI, NJ = Geo::NJ, KS = Geo::KS, ND = Geo::ND;
   // Objects of their own, so that the compiler knows that reads of one do not
   // wait for loads into another.
@@ -667,64 +665,48 @@ __global__ void __launch_bounds__(kPgThreads, KT <= 4 ? 2 : 1) paged_chunk_kerne
     };
 
     // The lane's query rows, their last keys, and the wave's tokens.
-    uint4 qx[RG][KS];
-    int tok[RG];
+    int qt, qh;
+    const bool own = u.row(32 * wave + row, qt, qh);
+    uint4 qx[KS];
+    const char *qp = p.q + (own ? qt : u.row0) * p.q_t + (own ? qh : u.head0) * p.q_h + 16 * hf;
 #pragma unroll
-    for (int g = 0; g < RG; ++g) {
-      int qt, qh;
-      const bool own = u.row((wave * RG + g) * 32 + row, qt, qh);
-      const char *qp = p.q + (own ? qt : u.row0) * p.q_t + (own ? qh : u.head0) * p.q_h + 16 * hf;
-#pragma unroll
-      for (int st = 0; st < KS; ++st) qx[g][st] = load16(qp + 32 * st);
-      tok[g] = own ? qt - u.row0 : 0;
-    }
-    const bool active = wave * RG * 32 < u.tokens * u.gw;
-    const int tok_a = min(wave * RG * 32 / u.gw, u.tokens - 1);
-    const int tok_z = min(((wave + 1) * RG * 32 - 1) / u.gw, u.tokens - 1);
+    for (int st = 0; st < KS; ++st) qx[st] = load16(qp + 32 * st);
+    const int tok = own ? qt - u.row0 : 0;
+    const bool active = 32 * wave < u.tokens * u.gw;
+    const int tok_a = min(32 * wave / u.gw, u.tokens - 1), tok_z = min((32 * wave + 31) / u.gw, u.tokens - 1);
 
-    f32x16_t o[RG][ND] = {};
-    float m_run[RG], l_lane[RG];
-#pragma unroll
-    for (int g = 0; g < RG; ++g) {
-      m_run[g] = -INFINITY;
-      l_lane[g] = 0.f;
-    }
+    f32x16_t o[ND] = {};
+    float m_run = -INFINITY, l_lane = 0.f;  // l_lane: this lane's share of the row sum
 
     // Hidden keys' scores of tile t become -inf.
-    auto hide = [&](f32x16_t(&s)[RG][2], int t, uint64_t there) {
+    auto hide = [&](f32x16_t(&s)[2], int t, uint64_t there) {
       const int key0 = t << kChunkTileShift;
       const bool edge = key0 + 63 > u.last0 + tok_a || (p.sh.window > 0 && key0 + p.sh.window <= u.last0 + tok_z);
       if (!edge && there == ~uint64_t(0)) return;
+      // Keys [lo, hi) of the tile; a window as long as the keys hides none.
+      const int hi = u.last0 + tok + 1 - key0, lo = p.sh.window > 0 && hi > 0 ? hi - p.sh.window : 0;
+      uint64_t v = hi >= 64 ? ~uint64_t(0) : hi <= 0 ? 0 : (uint64_t(1) << hi) - 1;
+      if (lo > 0) v &= lo >= 64 ? 0 : ~uint64_t(0) << lo;
+      v = (v & there) >> (4 * hf);
 #pragma unroll
-      for (int g = 0; g < RG; ++g) {
-        // Keys [lo, hi) of the tile; a window as long as the keys hides none.
-        const int hi = u.last0 + tok[g] + 1 - key0, lo = p.sh.window > 0 && hi > 0 ? hi - p.sh.window : 0;
-        uint64_t v = hi >= 64 ? ~uint64_t(0) : hi <= 0 ? 0 : (uint64_t(1) << hi) - 1;
-        if (lo > 0) v &= lo >= 64 ? 0 : ~uint64_t(0) << lo;
-        v = (v & there) >> (4 * hf);
+      for (int sub = 0; sub < 2; ++sub) {
+        const uint32_t bits = (uint32_t)(v >> (32 * sub));
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-          const uint32_t bits = (uint32_t)(v >> (32 * sub));
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!(bits & (1u << (8 * (i >> 2) + (i & 3))))) s[g][sub][i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; ++i)
+          if (!(bits & (1u << (8 * (i >> 2) + (i & 3))))) s[sub][i] = -INFINITY;
       }
     };
-    // Raises the running maxima (and rescales the sums) where a score exceeds
-    // them by more than 2^kPgSlack.
-    auto raise = [&](const float (&x)[RG]) {
+    // Raises the running maximum (and rescales the sums) where a score exceeds
+    // it by more than 2^kPgSlack.
+    auto raise = [&](float x) {
+      if (!__ballot(x * cc > m_run + kPgSlack)) return;
+      const float mt = half_wave_max(x) * cc;
+      const float m_new = mt > m_run + kPgSlack ? mt : m_run;
+      const float a = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      l_lane *= a;
 #pragma unroll
-      for (int g = 0; g < RG; ++g) {
-        if (!__ballot(x[g] * cc > m_run[g] + kPgSlack)) continue;
-        const float mt = half_wave_max(x[g]) * cc;
-        const float m_new = mt > m_run[g] + kPgSlack ? mt : m_run[g];
-        const float a = m_run[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[g] - m_new);
-        l_lane[g] *= a;
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) o[g][dt] *= a;
-        m_run[g] = m_new;
-      }
+      for (int dt = 0; dt < ND; ++dt) o[dt] *= a;
+      m_run = m_new;
     };
     auto k_op = [&](const char *kb, int i) {
       return *reinterpret_cast<const uint4 *>(kb + (kaddr ^ ((i % KS) << 5)) + (i / KS) * 32 * CP * 16);
@@ -735,12 +717,6 @@ __global__ void __launch_bounds__(kPgThreads, KT <= 4 ? 2 : 1) paged_chunk_kerne
       const uint2 hi =
           __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t *)(at + 8 * CP * 16)));
       return make_uint4(lo.x, lo.y, hi.x, hi.y);
-    };
-    auto top = [&](const f32x16_t(&s)[RG][2], int g) {
-      float x = s[g][0][0];
-#pragma unroll
-      for (int i = 1; i < 32; ++i) x = fmaxf(x, s[g][i >> 4][i & 15]);
-      return x;
     };
     auto arrived = [&] {
       asm volatile("" ::: "memory");
@@ -760,24 +736,28 @@ __global__ void __launch_bounds__(kPgThreads, KT <= 4 ? 2 : 1) paged_chunk_kerne
     locate(part.t0 + 1, pg1, off1, th1);
     if (part.t0 + 1 < part.t1) load(off1, th1, kbase, kb1, kc0, kc1);
     arrived();
-    f32x16_t sa[RG][2] = {}, sb[RG][2];
+    f32x16_t sa[2] = {}, sb[2];
     if (active) {
+      constexpr int NR = 2 * KS, kAhead = NR < 6 ? NR : 6;
+      uint4 ka[NR];
 #pragma unroll
-      for (int i = 0; i < 2 * KS; ++i) {
-        const uint4 a = k_op(kb0, i);
+      for (int i = 0; i < kAhead; ++i) ka[i] = k_op(kb0, i);
 #pragma unroll
-        for (int g = 0; g < RG; ++g) sa[g][i / KS] = mfma_32x32x16<DT>(a, qx[g][i % KS], sa[g][i / KS]);
+      for (int i = 0; i < NR; ++i) {
+        if (i + kAhead < NR) ka[i + kAhead] = k_op(kb0, i + kAhead);
+        sa[i / KS] = mfma_32x32x16<DT>(ka[i], qx[i % KS], sa[i / KS]);
+        __builtin_amdgcn_sched_barrier(0);
       }
       hide(sa, part.t0, th0);
-      float x[RG];
+      float x = sa[0][0];
 #pragma unroll
-      for (int g = 0; g < RG; ++g) x[g] = top(sa, g);
+      for (int i = 1; i < 32; ++i) x = fmaxf(x, sa[i >> 4][i & 15]);
       raise(x);
     }
     int t = part.t0;
     // One tile: sc its scores, vr its values; sn, kr the next tile's; kw, vw
     // the buffers of the tiles behind those.
-    auto step = [&](f32x16_t(&sc)[RG][2], f32x16_t(&sn)[RG][2], const char *kr, const char *vr, char *kw, char *vw) {
+    auto step = [&](f32x16_t(&sc)[2], f32x16_t(&sn)[2], const char *kr, const char *vr, char *kw, char *vw) {
       arrived();
       // The pages' numbers first: behind new loads they would wait for those.
       int64_t off2;
@@ -787,60 +767,52 @@ __global__ void __launch_bounds__(kPgThreads, KT <= 4 ? 2 : 1) paged_chunk_kerne
       if (t + 2 < part.t1) load(off2, th2, kbase, kw, kc0, kc1);
       const int pg3 = lookup(t + 3);
       if (active) {
-        float m_neg[RG];
-        uint4 pb[RG][4];
-#pragma unroll
-        for (int g = 0; g < RG; ++g) m_neg[g] = m_run[g] == -INFINITY ? 0.f : -m_run[g];
         // Scores of the next tile (of no tile behind the last: not used)
         // beside this one's probabilities, 2^(cc s - m), rounded to the dtype
         // as operands; their sums keep the fp32 values.
-        constexpr int NR = 2 * KS, kAhead = NR < 3 ? NR : 3, PAIRS = 16 * RG;  // pairs of a lane's scores
+        constexpr int NR = 2 * KS, kAhead = NR < 3 ? NR : 3;
+        const float m_neg = m_run == -INFINITY ? 0.f : -m_run;
         uint4 ka[NR];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) ka[i] = k_op(kr, i);
-        uint32_t w[RG][16];
+        // This phase has the vector instructions: its wave goes before the one
+        // that shares the SIMD, whose matrix instructions fill in (4096 tokens
+        // over 8192 keys 181 -> 173 us; the other phase first 175, both 177).
+        __builtin_amdgcn_s_setprio(1);
+        uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
           if (i + kAhead < NR) ka[i + kAhead] = k_op(kr, i + kAhead);
+          sn[i / KS] = mfma_32x32x16<DT>(ka[i], qx[i % KS], i % KS == 0 ? f32x16_t{} : sn[i / KS]);
 #pragma unroll
-          for (int g = 0; g < RG; ++g)
-            sn[g][i / KS] = mfma_32x32x16<DT>(ka[i], qx[g][i % KS], i % KS == 0 ? f32x16_t{} : sn[g][i / KS]);
-#pragma unroll
-          for (int e = PAIRS * i / NR; e < PAIRS * (i + 1) / NR; ++e) {
-            const int g = e >> 4, at = 2 * (e & 15);
-            const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[g][at >> 4][at & 15], cc, m_neg[g]));
-            const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[g][at >> 4][(at & 15) + 1], cc, m_neg[g]));
-            l_lane[g] += e0;
-            l_lane[g] += e1;
-            w[g][e & 15] = pack2<DT>(e0, e1);
-            stay(w[g][e & 15]);
+          for (int e = 16 * i / NR; e < 16 * (i + 1) / NR; ++e) {
+            const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[e >> 3][2 * (e & 7)], cc, m_neg));
+            const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[e >> 3][2 * (e & 7) + 1], cc, m_neg));
+            l_lane += e0;
+            l_lane += e1;
+            w[e] = pack2<DT>(e0, e1);
+            stay(w[e]);
           }
-#pragma unroll
-          for (int g = 0; g < RG; ++g) stay(l_lane[g]);
+          stay(l_lane);
           __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
+        uint4 pb[4];
 #pragma unroll
-        for (int g = 0; g < RG; ++g)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) pb[g][k] = make_uint4(w[g][4 * k], w[g][4 * k + 1], w[g][4 * k + 2], w[g][4 * k + 3]);
+        for (int k = 0; k < 4; ++k) pb[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
         constexpr int NV = 4 * ND, vAhead = NV < 4 ? NV : 4;
         uint4 va[NV];
 #pragma unroll
         for (int i = 0; i < vAhead; ++i) va[i] = v_op(vr, i / ND, i % ND);
         if (t + 1 < part.t1) hide(sn, t + 1, th1);
-        float x[RG];
-#pragma unroll
-        for (int g = 0; g < RG; ++g) x[g] = sn[g][0][0];
+        float x = sn[0][0];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           if (i + vAhead < NV) va[i + vAhead] = v_op(vr, (i + vAhead) / ND, (i + vAhead) % ND);
+          o[i % ND] = mfma_32x32x16<DT>(va[i], pb[i / ND], o[i % ND]);
 #pragma unroll
-          for (int g = 0; g < RG; ++g) {
-            o[g][i % ND] = mfma_32x32x16<DT>(va[i], pb[g][i / ND], o[g][i % ND]);
-#pragma unroll
-            for (int e = 32 * i / NV; e < 32 * (i + 1) / NV; ++e) x[g] = fmaxf(x[g], sn[g][e >> 4][e & 15]);
-            stay(x[g]);
-          }
+          for (int e = 32 * i / NV; e < 32 * (i + 1) / NV; ++e) x = fmaxf(x, sn[e >> 4][e & 15]);
+          stay(x);
           __builtin_amdgcn_sched_barrier(0);
         }
         if (t + 1 < part.t1) raise(x);
@@ -856,34 +828,52 @@ __global__ void __launch_bounds__(kPgThreads, KT <= 4 ? 2 : 1) paged_chunk_kerne
       step(sb, sa, kb0, vb1, kb1, vb0);
     }
 
+    // The wave's rows, through a tile's LDS: a store then takes whole rows
+    // (from the accumulators it would take 32 bytes of each of 32 rows).
+    __syncthreads();  // every wave has read the last tile
+    int ln = lane;  // hidden from the compiler, which would otherwise keep the addresses formed from it
+    stay(ln);       // below in registers through every tile
+    const int er = ln & 31, eh = ln >> 5;
+    int qt_e, qh_e;
+    const bool own_e = u.row(32 * wave + er, qt_e, qh_e);
+    char *rows = wave == 0 ? kb0 : wave == 1 ? kb1 : wave == 2 ? vb0 : vb1;
+    constexpr int RC = D / 4;  // 16-byte chunks of an fp32 row; chunk c of row r at c ^ (r % 8)
+    static_assert(32 * RC * 16 <= Geo::TILE, "a wave's rows fit a tile");
 #pragma unroll
-    for (int g = 0; g < RG; ++g) {
-      const float l_row = half_wave_sum(l_lane[g]);
-      int qt, qh;
-      if (!u.row((wave * RG + g) * 32 + row, qt, qh)) continue;
-      if (part.partial >= 0) {
-        const int64_t sr = (int64_t)part.partial * p.sh.rows + (wave * RG + g) * 32 + row;
-        float *po = p.ws_o + sr * D + 4 * hf;
+    for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt)
+      for (int n = 0; n < 4; ++n)
+        *reinterpret_cast<f32x4_t *>(rows + (er * RC + ((8 * dt + 2 * n + eh) ^ (er & 7))) * 16) =
+            f32x4_t{o[dt][4 * n], o[dt][4 * n + 1], o[dt][4 * n + 2], o[dt][4 * n + 3]};
+    const float l_row = half_wave_sum(l_lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    auto chunk_of = [&](int r, int c) { return *reinterpret_cast<const f32x4_t *>(rows + (r * RC + (c ^ (r & 7))) * 16); };
+    if (part.partial >= 0) {
+      const int64_t sr = (int64_t)part.partial * p.sh.rows + 32 * wave;
+      if (own_e && eh == 0) {
+        p.ws_m[sr + er] = m_run;
+        p.ws_l[sr + er] = l_row;
+      }
+      float *po = p.ws_o + sr * D;
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
-            *reinterpret_cast<f32x4_t *>(po + 32 * dt + 8 * n) =
-                f32x4_t{o[g][dt][4 * n], o[g][dt][4 * n + 1], o[g][dt][4 * n + 2], o[g][dt][4 * n + 3]};
-        if (hf == 0) {
-          p.ws_m[sr] = m_run[g];
-          p.ws_l[sr] = l_row;
-        }
-      } else {
-        // A row that sees no key gets zeros.
-        const float inv = l_row > 0.f ? 1.f / l_row : 0.f;
-        const int64_t at = ((int64_t)qt * p.hq + qh) * D + 4 * hf;
+      for (int i0 = 0; i0 < 32 * RC; i0 += 64) {
+        const int i = i0 + ln, r = i / RC;
+        if (32 * wave + r < u.tokens * u.gw) *reinterpret_cast<f32x4_t *>(po + 4 * i) = chunk_of(r, i - r * RC);
+      }
+    } else {
+      // A row that sees no key gets zeros.
+      const float inv = l_row > 0.f ? 1.f / l_row : 0.f;
+      const int64_t at = own_e ? ((int64_t)qt_e * p.hq + qh_e) * D : -1;
 #pragma unroll
-        for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-            store4<DT>(p.out, at + 32 * dt + 8 * n,
-                       f32x4_t{o[g][dt][4 * n], o[g][dt][4 * n + 1], o[g][dt][4 * n + 2], o[g][dt][4 * n + 3]} * inv);
+      for (int i0 = 0; i0 < 32 * RC / 2; i0 += 64) {
+        const int i = i0 + ln, r = i / (RC / 2), c = 2 * (i - r * (RC / 2));
+        const float f = __shfl(inv, r, 64);
+        const int64_t to = __shfl(at, r, 64);
+        const f32x4_t x = chunk_of(r, c) * f, y = chunk_of(r, c + 1) * f;
+        if (to >= 0)
+          *reinterpret_cast<uint4 *>(p.out + (to + 4 * c) * 2) =
+              make_uint4(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]), pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]));
       }
     }
     if (wk.w < wk.w_end) {
@@ -998,9 +988,8 @@ struct PagedPlan {
   size_t m_off, l_off, o_off, total;  // workspace: cuts, then these
 };
 
-constexpr int chunk_groups(int D) { return 1; }
 constexpr int chunk_load_rows(int D) { return D <= 32 ? 16 : D <= 64 ? 8 : D <= 128 ? 4 : 2; }
-constexpr int chunk_rows(int D) { return 128 * chunk_groups(D); }
+constexpr int kChunkRows = 128;
 
 static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
   const kiv_paged_cache_t &c = a.cache;
@@ -1013,7 +1002,7 @@ static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
   // a tile's rows within 2 GiB.
   w.chunk = c.dtype != KIV_DTYPE_F32 && (int64_t)std::min(b.max_q_len, b.total_q) * G > kRowsOfUnit &&
             c.page_size % chunk_load_rows(c.head_dim) == 0 && c.stride[2] >= 0 && c.stride[2] < (1 << 24);
-  const int rows = w.chunk ? chunk_rows(c.head_dim) : kRowsOfUnit, shift = w.chunk ? kChunkTileShift : kRowsTileShift;
+  const int rows = w.chunk ? kChunkRows : kRowsOfUnit, shift = w.chunk ? kChunkTileShift : kRowsTileShift;
   const int window = std::min(a.window, 1 << 30);  // no table is as long
   w.sh = PagedShape::of(b.total_q, c.num_kv_heads, G, rows, cap, shift, window, false);
   // More than the call's units and tiles, by what the host knows of them.
@@ -1146,7 +1135,7 @@ int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream
       constexpr int DTV = decltype(dtc)::value;
       if constexpr (DTV != DT_F32) {
         if (w.chunk)
-          hipLaunchKernelGGL((paged_chunk_kernel<DTV, DV / 32, chunk_groups(DV)>), grid, dim3(kPgThreads), 0, st, p);
+          hipLaunchKernelGGL((paged_chunk_kernel<DTV, DV / 32>), grid, dim3(kPgThreads), 0, st, p);
       }
       if (!w.chunk) hipLaunchKernelGGL((paged_rows_kernel<DTV, DV>), grid, dim3(kPgThreads), 0, st, p);
       if (w.total == 0) return;
