@@ -273,10 +273,17 @@ def layout(t: torch.Tensor) -> Layout:
     key = (t.shape, t.stride(), t.dtype)
     got = _layouts.get(key)
     if got is None:
-        got = Layout(key[0], key[1], t.element_size())
-        if len(_layouts) < 4096:
-            _layouts[key] = got
+        got = remember(_layouts, key, Layout(key[0], key[1], t.element_size()))
     return got
+
+
+def remember(known: dict, key, value):
+    """Keep what a key's shapes give; a full table starts again (steps of a
+    serving loop bring ever new token counts)."""
+    if len(known) >= 4096:
+        known.clear()
+    known[key] = value
+    return value
 
 
 def stream_ptr(device: torch.device) -> int:

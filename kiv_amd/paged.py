@@ -61,16 +61,24 @@ class PagedKVCache:
             raise ValueError("the paged cache lives on a GPU")
         out_rows(k, k, "K pages")
         out_rows(v, v, "V pages")
-        self.k, self.v = k, v
+        self._k, self._v = k, v
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype, self.device = k.dtype, k.device
         self._args = nat.PagedCacheArgs(k.data_ptr(), v.data_ptr(), nat.layout(k).strides, self.num_pages,
                                         self.page_size, self.num_kv_heads, self.head_dim, nat.dtype_code(k.dtype), 0)
         self._geometry = (tuple(k.shape), k.stride(), k.dtype)
 
+    @property
+    def k(self) -> torch.Tensor:
+        return self._k
+
+    @property
+    def v(self) -> torch.Tensor:
+        return self._v
+
     def memory_bytes(self) -> int:
         """Bytes of the pool's K and V rows."""
-        return 2 * self.k.numel() * self.k.element_size()
+        return 2 * self._k.numel() * self._k.element_size()
 
 
 class PagedBatch:
@@ -110,13 +118,25 @@ class PagedBatch:
                 raise ValueError(f"{name} must be on the batch's GPU")
             if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
                 raise ValueError(f"{name} must have unit stride")
-        self.block_table, self.kv_len, self.cu_q = block_table, kv_len, cu_q
+        self._block_table, self._kv_len, self._cu_q = block_table, kv_len, cu_q
         self.num_seqs, self.device = S, block_table.device
         big = 2**31 - 1
         self._args = nat.PagedBatchArgs(
             cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0) if S > 1 else 0, S, W, 0,
             big if max_q_len is None else min(max_q_len, big), big if max_kv_len is None else min(max_kv_len, big), 0)
         self._geometry = (S, W, self._args.max_q_len, self._args.max_kv_len, self.device)
+
+    @property
+    def block_table(self) -> torch.Tensor:
+        return self._block_table
+
+    @property
+    def kv_len(self) -> torch.Tensor:
+        return self._kv_len
+
+    @property
+    def cu_q(self) -> torch.Tensor:
+        return self._cu_q
 
 
 def _packed_layout(t: torch.Tensor, name: str, cache: PagedKVCache, heads: int | None) -> nat.Layout:
@@ -141,7 +161,8 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
     [tokens] or, with ``rotary.axes``, [axes, tokens]; None turns each token
     by its key index.  With q [tokens, Hq, D] the queries are normed
     (``q_norm``) and turned in the same launch, into ``q_out`` (new by
-    default; may be q); returns it, else None.  Rows past the last sequence
+    default; may be q, and must not overlap it otherwise); returns it, else
+    None.  Rows past the last sequence
     are left alone, in the pages and in ``q_out``; a token whose page is not
     there is dropped.
     """
@@ -150,9 +171,7 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
            None if q is None else (q.shape, q.stride(), q.dtype))
     plan = _append_plans.get(key)
     if plan is None:
-        plan = _append_plan(cache, k, v, q)
-        if len(_append_plans) < 4096:
-            _append_plans[key] = plan
+        plan = nat.remember(_append_plans, key, _append_plan(cache, k, v, q))
     template, T, copy = plan
     dev, D = cache.device, cache.head_dim
     if k.device != dev or v.device != dev or batch.device != dev or (q is not None and q.device != dev):
@@ -238,9 +257,7 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
     key = (query.shape, query.stride(), query.dtype, window, cache._geometry, batch._geometry)
     plan = _attention_plans.get(key)
     if plan is None:
-        plan = _attention_plan(query, cache, batch, window)
-        if len(_attention_plans) < 4096:
-            _attention_plans[key] = plan
+        plan = nat.remember(_attention_plans, key, _attention_plan(query, cache, batch, window))
     template, need, T, copy = plan
     args = nat.PagedAttentionArgs.from_buffer_copy(template)
     args.cache, args.batch = cache._args, batch._args

@@ -35,10 +35,14 @@ class HeadNorm:
             raise ValueError("a norm without a weight has no offset")
         if not eps >= 0.0:
             raise ValueError(f"norm epsilon must not be negative, got {eps}")
-        self.weight = weight
+        self._weight = weight
         self.eps = eps
         self._at = None if weight is None else (weight.shape[0], weight.device)
         self._args = nat.HeadNormArgs(nat.ptr(weight), eps, 1)
+
+    @property
+    def weight(self) -> torch.Tensor | None:
+        return self._weight
 
     def check(self, head_dim: int, device: torch.device) -> nat.HeadNormArgs:
         at = self._at
@@ -58,7 +62,8 @@ class Rotary:
     scale        factor of the cosines and sines.
     axes         [rot_dim / 2] integers: the position axis each pair follows
                  (images and video: time, height, width); positions then have
-                 a leading axis dimension.
+                 a leading axis dimension.  A number outside it means its
+                 nearest axis.
     """
 
     def __init__(self, inv_freq: torch.Tensor, interleaved: bool = False, scale: float = 1.0,
@@ -75,14 +80,20 @@ class Rotary:
             if axes.is_floating_point() or axes.dtype == torch.bool:
                 raise TypeError(f"axes must be integers, not {axes.dtype}")
             axes = axes.to(torch.int32).contiguous()
-        self.inv_freq = inv_freq.contiguous()
-        self.axes = axes
-        self.interleaved = bool(interleaved)
-        self.scale = float(scale)
+        self._inv_freq = inv_freq.detach().contiguous()
+        self._axes = axes
         self.rot_dim = 2 * inv_freq.shape[0]
         self.device = inv_freq.device
-        self._args = nat.RotaryArgs(self.inv_freq.data_ptr(), nat.ptr(axes), None, nat._I64x3(), 0, 1, self.rot_dim,
-                                    int(self.interleaved), self.scale, 0)
+        self._args = nat.RotaryArgs(self._inv_freq.data_ptr(), nat.ptr(axes), None, nat._I64x3(), 0, 1, self.rot_dim,
+                                    int(bool(interleaved)), float(scale), 0)
+
+    @property
+    def inv_freq(self) -> torch.Tensor:
+        return self._inv_freq
+
+    @property
+    def axes(self) -> torch.Tensor | None:
+        return self._axes
 
     def fill(self, dst: nat.RotaryArgs, positions: torch.Tensor | None, batch: int, tokens: int,
              device: torch.device, batched: bool) -> None:
@@ -90,7 +101,7 @@ class Rotary:
         or either behind an axis dimension."""
         if self.device != device:
             raise ValueError(f"inv_freq is on {self.device}, rows on {device}")
-        lead = self.axes is not None
+        lead = self._axes is not None
         if positions is None:
             if lead:
                 raise ValueError("a rotation with several axes needs positions")
@@ -100,9 +111,7 @@ class Rotary:
         key = (positions.shape, positions.stride(), positions.dtype, lead, batched, batch, tokens)
         got = _position_layouts.get(key)
         if got is None:
-            got = _position_layout(*key)
-            if len(_position_layouts) < 4096:
-                _position_layouts[key] = got
+            got = nat.remember(_position_layouts, key, _position_layout(*key))
         dst.position_stride, dst.position_bytes, dst.num_axes = got
         dst.positions = positions.data_ptr()
 
@@ -164,7 +173,8 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor |
 
     positions: [T], [B, T] or, with ``rotary.axes``, [axes, T] or
     [axes, B, T]; int32 or int64.  ``q_out`` / ``k_out`` may be the inputs
-    themselves; by default they are new tensors in the inputs' memory order.
+    themselves (and must not overlap them otherwise); by default they are new
+    tensors in the inputs' memory order.
     fp32, fp16 and bf16; head_dim a multiple of 16 bytes up to 512, the
     rotated width of 32 bytes.  Returns (q_out, k_out).
     """
@@ -175,9 +185,7 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor |
     key = (q.shape, q.stride(), q.dtype, None if k is None else (k.shape, k.stride(), k.dtype))
     plan = _plans.get(key)
     if plan is None:
-        plan = _plan(q, k)
-        if len(_plans) < 4096:
-            _plans[key] = plan
+        plan = nat.remember(_plans, key, _plan(q, k))
     template, B, T, D, copy_q, copy_k = plan
     args = nat.NormRopeArgs.from_buffer_copy(template)
     at = q.data_ptr()

@@ -340,3 +340,30 @@ def test_paged_attention_refusals(cuda):
     empty = PagedBatch(batch.block_table[:0], batch.kv_len[:0])
     assert paged_attention(dq[:0], cache, empty, 1.0).shape == (0, 4, 64)
     assert paged_attention(dq[:0], cache, batch, 1.0).shape == (0, 4, 64)
+
+
+def test_handles_keep_their_tensors(cuda):
+    """The kernels read through addresses taken at construction: the tensors
+    behind them cannot be swapped, and live as long as the handle."""
+    g = torch.Generator().manual_seed(59)
+    cache, batch, table, cu, q, k, v = setup(g, BF16, [1], [40], 4, 2, 64, 16, False, cuda)
+    for obj, name in ((batch, "kv_len"), (batch, "cu_q"), (batch, "block_table"), (cache, "k"), (cache, "v"),
+                      (HeadNorm(), "weight"), (Rotary(torch.ones(32, device=cuda)), "inv_freq")):
+        with pytest.raises(AttributeError):
+            setattr(obj, name, None)
+    handle = PagedBatch(table.to(cuda), torch.tensor([40], dtype=torch.int32, device=cuda),
+                        torch.tensor([0, 1], dtype=torch.int32, device=cuda))
+    junk = [torch.full((n,), 7, dtype=torch.int32, device=cuda) for n in (1, 2, 4) * 20]
+    verify(paged_attention(q.to(cuda), cache, handle, 0.125), q, k, v, table, [40], cu, 0.125)
+    del junk
+
+
+def test_many_shapes_in_turn(cuda):
+    """Token counts that change from call to call: no shape's arguments serve
+    another's."""
+    g = torch.Generator().manual_seed(61)
+    cache, batch, table, cu, q, k, v = setup(g, BF16, [37], [400], 8, 2, 64, 16, False, cuda)
+    dq = q.to(cuda)
+    for n in (1, 2, 3, 5, 8, 37, 2, 1):
+        b = PagedBatch(batch.block_table, batch.kv_len, torch.tensor([0, n], dtype=torch.int32, device=cuda))
+        verify(paged_attention(dq[37 - n:], cache, b, 0.125), q[37 - n:], k, v, table, [400], [0, n], 0.125)
