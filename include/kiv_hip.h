@@ -1,5 +1,6 @@
 /*
- * kiv_hip.h - C ABI of the MI355X (gfx950) tiered-KV-cache decode path.
+ * kiv_hip.h - C ABI of the MI355X (gfx950) tiered-KV-cache decode path, and
+ * of a paged cache beside it (last part).
  *
  * One opaque store per independent KV layer holds that layer's cold tier:
  *   - page summaries (mean of the page's post-RoPE K rows) in HBM,

@@ -28,7 +28,7 @@ class HeadNorm:
                 raise ValueError(f"norm weight must be [head_dim], got {tuple(weight.shape)}")
             if not weight.is_cuda:
                 raise ValueError("norm weight must be on a GPU")
-            weight = weight.detach().float().clone().contiguous()
+            weight = weight.detach().to(torch.float32, copy=True).contiguous()
             if offset:
                 weight += offset
         elif offset:
