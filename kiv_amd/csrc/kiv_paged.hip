@@ -184,7 +184,7 @@ struct PagedWork {
   // order stays below by the host's check).
   __device__ __forceinline__ bool deal(const PagedAttnParams &p, int total, float ftotal) {
     if (total <= 0 || ftotal > 2.1e9f) return false;
-    shares = PagedShares::deal(total, p.blocks);
+    shares = PagedShares::deal(total, p.blocks, p.sh.whole);
     if ((int)blockIdx.x >= shares.n) return false;
     // Blocks are dealt to the eight dies in turn: a die takes neighbouring
     // shares, which read the same keys through its L2.
@@ -268,21 +268,22 @@ struct PagedPart {
       ++wk.w;
       return;
     }
-    const int ue = wk.us + n, end = min(wk.w_end, ue);
-    t0 = first + wk.w - wk.us;
-    t1 = first + end - wk.us;
-    const bool begins = wk.w == wk.us, ends = end == ue;
-    partial = begins && ends ? -1 : begins ? 2 * wk.id + 1 : 2 * wk.id;
+    const int end = min(wk.w_end, wk.us + p.sh.fixed + n);
+    const int before = p.sh.tiles_before(wk.w - wk.us), upto = p.sh.tiles_before(end - wk.us);
+    t0 = first + before;
+    t1 = first + upto;  // t0 where the share ends in the unit's fixed weight: the next share has its first tile
+    partial = before > 0 ? 2 * wk.id : upto < n ? 2 * wk.id + 1 : -1;
     wk.w = end;
   }
 };
 
-// The cut in front of block id's share, if the block before it began the unit.
+// The cut in front of block id's share, if the block before it has the unit's
+// first tile.
 __device__ __forceinline__ void paged_write_cut(const PagedAttnParams &p, const PagedWork &wk, const PagedUnit &u) {
   if (!p.cuts || threadIdx.x != 0) return;
   PagedCut c = {u.row0, u.tokens, u.head0, u.heads, -1, {0, 0, 0}};
-  if (!p.sh.whole && wk.w > wk.us && wk.us >= wk.shares.start(wk.id - 1))
-    c.last = wk.shares.block_of(wk.us + p.sh.tiles(u.k0, u.k1) - 1);
+  if (p.sh.tiles_before(wk.w - wk.us) > 0 && p.sh.tiles_before(wk.shares.start(wk.id - 1) - wk.us) == 0)
+    c.last = wk.shares.block_of(wk.us + p.sh.fixed + p.sh.tiles(u.k0, u.k1) - 1);
   p.cuts[wk.id] = c;
 }
 __device__ __forceinline__ void paged_no_cut(const PagedAttnParams &p, int id) {
@@ -338,6 +339,7 @@ paged_rows_kernel(PagedAttnParams p) {
     if (head) paged_write_cut(p, wk, u);
     head = false;
     const PagedPart part(p, wk, u);
+    if (part.t0 == part.t1) break;  // the share ends before the unit's first tile
     // The lane's query row (rows the unit has not repeat its first).
     int qt, qh;
     const bool own = u.row(col, qt, qh);
@@ -608,6 +610,7 @@ __global__ void __launch_bounds__(kPgThreads, KT <= 4 ? 2 : 1) paged_chunk_kerne
     if (head) paged_write_cut(p, wk, u);
     head = false;
     const PagedPart part(p, wk, u);
+    if (part.t0 == part.t1) break;  // the share ends before the unit's first tile
     const int32_t *table = p.table + wk.b * p.table_stride;
     const char *kbase = p.k + wk.kvh * p.head_b, *vbase = p.v + wk.kvh * p.head_b;
 
@@ -975,8 +978,17 @@ __global__ void __launch_bounds__(kPgThreads) paged_combine_kernel(PagedAttnPara
 
 // ------------------------------------------------------------------- host
 // Units of at most this many tiles (by the host's bound of the keys) are never
-// divided: one launch, no partial rows.
-constexpr int kWholeTiles = 4;
+// divided: one launch, no partial rows.  Chunks: 512 tokens of 32 heads over 8
+// 18 us whole, 27 divided; 1000 (16 tiles) 29, 35; 1500 of 12 over 2 (24
+// tiles, few units) 39, 33; above head_dim 128, one block a compute unit, 1000
+// tokens 44, 32.  Units of 16 rows: 8 sequences of 1000 keys (8 tiles) 18.4,
+// 16.7; 301 keys 7, 11.
+static int whole_tiles(bool chunk, int head_dim) { return !chunk ? 4 : head_dim <= 128 ? 16 : 8; }
+// A unit's fixed cost in tiles.  Without it the shares of short units are the
+// longest: 8192 tokens of 12 heads over 2 305 us, 242 with three tiles, 230
+// with five, 236 with eight; 4096 of 28 over 4 224, 157, 148, 150.  Units of
+// 16 rows: one, two or three tiles alike, 3% less than none.
+constexpr int kChunkFixed = 5, kRowsFixed = 1;
 
 struct PagedPlan {
   PagedShape sh;
@@ -1007,11 +1019,12 @@ static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
             c.page_size % chunk_load_rows(c.head_dim) == 0 && c.stride[2] >= 0 && c.stride[2] < (1 << 24);
   const int rows = w.chunk ? kChunkRows : kRowsOfUnit, shift = w.chunk ? kChunkTileShift : kRowsTileShift;
   const int window = std::min(a.window, 1 << 30);  // no table is as long
-  w.sh = PagedShape::of(b.total_q, c.num_kv_heads, G, rows, cap, shift, window, false);
+  w.sh = PagedShape::of(b.total_q, c.num_kv_heads, G, rows, cap, shift, window, false,
+                        w.chunk ? kChunkFixed : kRowsFixed);
   // More than the call's units and tiles, by what the host knows of them.
   const int64_t units =
       ((int64_t)b.total_q / w.sh.tpu + std::min(b.num_seqs, b.total_q)) * w.sh.hpt * c.num_kv_heads;
-  w.weight = units * ((cap >> shift) + 2);
+  w.weight = units * ((cap >> shift) + 2 + w.sh.fixed);
   const int64_t keys = window > 0 ? std::min<int64_t>(most_keys, (int64_t)window + w.sh.tpu) : most_keys;
   const int64_t tiles = (keys >> shift) + 1;
   // Blocks that a compute unit holds at once: two, or one where a row's
@@ -1022,7 +1035,7 @@ static PagedPlan paged_plan(const kiv_paged_attention_args_t &a) {
   w.split = false;
   w.cuts_x = w.cuts_y = 0;
   w.m_off = w.l_off = w.o_off = w.total = 0;
-  if (tiles <= kWholeTiles) {
+  if (tiles <= whole_tiles(w.chunk, c.head_dim)) {
     w.sh.whole = 1;
     w.blocks = (int)std::min<int64_t>(4 * slots, units);
     return w;

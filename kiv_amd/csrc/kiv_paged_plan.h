@@ -47,8 +47,10 @@ struct PagedShape {
   int tile_shift;  // keys of a tile: 1 << tile_shift
   int window;      // 0: none
   int whole;       // a unit is never divided (its weight is one)
+  int fixed;       // tiles that a unit's first loads and its stores cost
 
-  static PagedShape of(int total_q, int hkv, int G, int rows, int cap, int tile_shift, int window, bool whole) {
+  static PagedShape of(int total_q, int hkv, int G, int rows, int cap, int tile_shift, int window, bool whole,
+                       int fixed) {
     PagedShape s;
     s.total_q = total_q;
     s.hkv = hkv;
@@ -61,6 +63,7 @@ struct PagedShape {
     s.tile_shift = tile_shift;
     s.window = window;
     s.whole = whole;
+    s.fixed = fixed;
     return s;
   }
   KIV_HD PagedSeq seq(int cu0, int cu1, int len) const {
@@ -87,12 +90,15 @@ struct PagedShape {
   // key has one, so that a block writes its rows.
   KIV_HD int first_tile(int k0) const { return k0 >> tile_shift; }
   KIV_HD int tiles(int k0, int k1) const { return k0 < k1 ? ((k1 - 1) >> tile_shift) - (k0 >> tile_shift) + 1 : 1; }
+  // A unit's weight: its fixed cost, then its tiles.
   KIV_HD int weight(const PagedSeq &s, int rt) const {
     if (whole) return 1;
     int k0, k1;
     keys(s, rt, k0, k1);
-    return tiles(k0, k1);
+    return fixed + tiles(k0, k1);
   }
+  // The unit's tiles before its weight w (counted from its first).
+  KIV_HD int tiles_before(int w) const { return w > fixed ? w - fixed : 0; }
 };
 
 // The weights 0 .. total - 1 in n shares, equal to within one: block i takes
@@ -100,12 +106,12 @@ struct PagedShape {
 struct PagedShares {
   int total, n, per, rem;
   // Dealt to at most `most` blocks, none without a weight; many blocks are a
-  // multiple of the eight dies.
-  KIV_HD static PagedShares deal(int total, int most) {
+  // multiple of the eight dies, unless a block then had a second whole unit.
+  KIV_HD static PagedShares deal(int total, int most, bool whole) {
     PagedShares s;
     const int m = total < most ? total : most;
     s.total = total;
-    s.n = m >= 64 ? m & ~7 : m;
+    s.n = m >= 64 && !(whole && m == total) ? m & ~7 : m;
     s.per = total / s.n;
     s.rem = total - s.per * s.n;
     return s;

@@ -57,7 +57,8 @@ static void walk(int seed) {
     len.push_back(pick(0, 20) ? pick(0, 4000) : pick(0, 1) ? -5 : 2147483647);
   }
   const int total_q = std::max(0, cu.back() + pick(-2, 3));
-  const PagedShape sh = PagedShape::of(total_q, hkv, G, rows, cap, shift, window, whole);
+  const int fixed = pick(0, 5);
+  const PagedShape sh = PagedShape::of(total_q, hkv, G, rows, cap, shift, window, whole, fixed);
   std::vector<Unit> units;
   long long total = 0;
   std::set<std::pair<int, int>> seen_rows;  // (packed row, head)
@@ -85,13 +86,13 @@ static void walk(int seed) {
         const int n = sh.tiles(k0, k1);
         for (int j : {k0, k1 - 1}) if (k0 < k1) EXPECT((j >> shift) >= sh.first_tile(k0) && (j >> shift) < sh.first_tile(k0) + n);
         units.push_back({s, b, h, rt, total, sh.weight(s, rt)});
-        EXPECT(sh.weight(s, rt) == (whole ? 1 : n));
+        EXPECT(sh.weight(s, rt) == (whole ? 1 : n + fixed));
         total += sh.weight(s, rt);
       }
   }
   if (total == 0) return;
   const int most = pick(1, 560);
-  const PagedShares shares = PagedShares::deal((int)total, most);
+  const PagedShares shares = PagedShares::deal((int)total, most, whole);
   EXPECT(shares.n >= 1 && shares.n <= most && shares.n <= total);
   EXPECT(shares.start(0) == 0 && shares.start(shares.n) == total);
   std::map<int, int> written;              // partial slot -> unit
@@ -104,22 +105,28 @@ static void walk(int seed) {
     EXPECT(shares.block_of(w) == i && shares.block_of(end - 1) == i);
     size_t u = 0;
     while (units[u].start + units[u].n <= w) ++u;
-    if (!whole && w > units[u].start && units[u].start >= shares.start(i - 1)) {
-      const int last = shares.block_of(units[u].start + units[u].n - 1);
+    auto before = [&](size_t v, long long x) {
+      return whole ? (int)(x - units[v].start) : sh.tiles_before((int)(x - units[v].start));
+    };
+    auto tiles = [&](size_t v) { return whole ? 1 : units[v].n - fixed; };
+    if (!whole && before(u, w) > 0 && before(u, shares.start(i - 1)) == 0) {
+      const int last = shares.block_of((int)(units[u].start + units[u].n - 1));
       merged[(int)u].push_back(2 * i - 1);
       for (int j = i; j <= last; ++j) merged[(int)u].push_back(2 * j);
     }
     for (; w < end; ++u) {
       const long long ue = units[u].start + units[u].n, e = std::min(end, ue);
-      const bool begins = w == units[u].start, ends = e == ue;
-      if (begins && ends) ++direct[u];
-      else EXPECT(written.insert({begins ? 2 * i + 1 : 2 * i, (int)u}).second);
-      taken[u] += e - w;
+      const int t0 = before(u, w), t1 = before(u, e);
+      EXPECT(t0 == taken[u]);
+      if (t0 == t1) { EXPECT(e == end); break; }
+      if (t0 == 0 && t1 == tiles(u)) ++direct[u];
+      else EXPECT(written.insert({t0 > 0 ? 2 * i : 2 * i + 1, (int)u}).second);
+      taken[u] += t1 - t0;
       w = e;
     }
   }
   for (size_t u = 0; u < units.size(); ++u) {
-    EXPECT(taken[u] == units[u].n);
+    EXPECT(taken[u] == (whole ? 1 : units[u].n - fixed));
     EXPECT(direct[u] + (long long)merged.count((int)u) == 1);
   }
   size_t read = 0;
