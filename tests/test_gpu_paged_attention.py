@@ -367,3 +367,29 @@ def test_many_shapes_in_turn(cuda):
     for n in (1, 2, 3, 5, 8, 37, 2, 1):
         b = PagedBatch(batch.block_table, batch.kv_len, torch.tensor([0, n], dtype=torch.int32, device=cuda))
         verify(paged_attention(dq[37 - n:], cache, b, 0.125), q[37 - n:], k, v, table, [400], [0, n], 0.125)
+
+
+@pytest.mark.parametrize("dtype,max_q", [(F32, 1), (BF16, 1), (BF16, None)])
+def test_more_whole_units_than_blocks(cuda, dtype, max_q):
+    """Over four thousand units of few keys: blocks take several each."""
+    g = torch.Generator().manual_seed(67)
+    lens = [1 + 7 * i % 40 for i in range(130)]
+    cache, batch, table, cu, q, k, v = setup(g, dtype, [1] * 130, lens, 32, 32, 32, 16, False, cuda)
+    b = PagedBatch(batch.block_table, batch.kv_len, batch.cu_q, max_q_len=max_q, max_kv_len=40)
+    verify(paged_attention(q.to(cuda), cache, b, 0.2), q, k, v, table, lens, cu, 0.2)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("qlens,lens", [([1], [1]), ([1, 0, 3, 1], [1, 0, 5, 130]), ([30, 1], [30, 300]),
+                                        ([1] * 9, [3] * 9), ([200], [4100])])
+def test_short_lengths_in_a_wide_table(cuda, dtype, qlens, lens):
+    """The table spans far more keys than the lengths reach: shares are dealt
+    where there is less work than blocks, some of them a unit's fixed weight
+    alone."""
+    g = torch.Generator().manual_seed(71)
+    cache, batch, table, cu, q, k, v = setup(g, dtype, qlens, lens, 8, 2, 64, 16, False, cuda)
+    wide = torch.full((len(lens), 3000), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    for max_q in (max(qlens), None):
+        b = PagedBatch(wide.to(cuda), batch.kv_len, batch.cu_q, max_q_len=max_q)
+        verify(paged_attention(q.to(cuda), cache, b, 0.125), q, k, v, wide, lens, cu, 0.125)
