@@ -23,9 +23,10 @@ LIBDIR = PKG / "_lib"
 LIB = LIBDIR / "libkiv_hip.so"
 SOURCES = ("kiv_store.hip", "kiv_retrieve.hip", "kiv_attention.hip", "kiv_prefill.hip", "kiv_rotary.hip",
            "kiv_paged.hip", "kiv_probe.hip")
-# Per-source flags.  The prefill attention keeps its MFMA accumulators in
-# ordinary VGPRs (the softmax rescales them every few tiles; in AGPRs every
-# tile would pay a copy in and out).
+# Per-source flags.  The prefill and the paged attention keep their MFMA
+# accumulators in ordinary VGPRs (the softmax rescales them every few tiles; in
+# AGPRs every tile would pay a copy in and out: the paged attention of 4096
+# tokens over 8192 keys 381 us against 263, at the step that was measured).
 EXTRA = {"kiv_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
          "kiv_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]}
 ARCH = os.environ.get("KIV_OFFLOAD_ARCH", "gfx950")

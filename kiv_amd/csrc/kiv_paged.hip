@@ -7,10 +7,11 @@
 // One pass over the keys with a running maximum and sum (base 2, fp32); the
 // query heads of one kv head are rows of one unit (kiv_paged_plan.h), so each
 // K and V row is read once for all of them.  The work of a call, in tiles of
-// keys, is dealt to the blocks in equal shares: a block finds its share from
-// the sequences' lengths itself (no launch, no host copy), takes its units
-// one after the other, and a unit that a share's end cuts is merged from
-// partial rows by paged_combine_kernel.
+// keys (a unit's first loads and stores count as some more), is dealt to the
+// blocks in equal shares: a block finds its share from the sequences' lengths
+// itself (no launch, no host copy), takes its units one after the other, and a
+// unit that a share's end cuts is merged from partial rows by
+// paged_combine_kernel.  Short units go whole, in one launch.
 //
 // paged_rows_kernel (single tokens, few rows, fp32): units of 16 rows, tiles
 // of 128 keys.  Each of a block's four waves takes 32 keys of a tile on its
@@ -22,7 +23,9 @@
 //   of both, and receives keys 4 (l / 16) + i of the sub-tile for row l % 16.
 //   O^T += V^T P^T: B is the lane's own probabilities, A the same keys of dim
 //   l % 16 from the LDS.
-// Bound: memory (each K and V byte is used by at most 16 rows).
+// Bound: memory (each K and V byte is used by at most 16 rows): 64 sequences
+// of up to 8192 keys, 28 heads over 4 of 128, 97 us (5.3 TB/s); one token over
+// a million keys 359 us (6.0 TB/s); both without the merge.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -94,7 +97,6 @@ __device__ __forceinline__ int paged_seq_weight(const PagedShape &sh, const Page
 __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams &p, int b) {
   return b < p.seqs ? p.sh.seq(p.cu[b], p.cu[b + 1], p.kv_len[b]) : PagedSeq{0, 0, 0};
 }
-__device__ __forceinline__ int64_t uniform_i64(int64_t x) { return (int64_t)uniform_u64((uint64_t)x); }
 
 // A block's place in the work: the unit it is at and what is left of its share.
 struct PagedWork {
@@ -554,6 +556,10 @@ paged_rows_kernel(PagedAttnParams p) {
 // One iteration forms the scores of the next tile beside the exponentials of
 // this one, then adds this tile's values beside the next one's maxima, so
 // that vector and matrix instructions alternate in one wave's stream.
+// Bound: neither unit is full (matrix cores busy 51% of the cycles): 4096 tokens
+// over 8192 keys, 12 heads over 2 of 128, 174 to 185 us with the merge, 840 to
+// 890 TFLOP/s; 1 PFLOP/s on long keys.  Two waves a SIMD: the registers hold no
+// third.
 template <int KT> struct ChunkGeom {
   static constexpr int D = 32 * KT, CPR = D / 8;
   static constexpr int CP = CPR <= 4 ? 4 : CPR <= 8 ? 8 : CPR <= 16 ? 16 : 32;  // chunks of an LDS row
@@ -891,7 +897,8 @@ __global__ void __launch_bounds__(kPgThreads, KT <= 4 ? 2 : 1) paged_chunk_kerne
 // A block takes the cuts of neighbouring shares; D / 4 threads a row, kCombineParts
 // parts of it in flight together.  SPLIT (units cut into many parts): a row a
 // block, its parts dealt to the block's groups of D / 4 threads, whose sums
-// meet in LDS; else a row a group.
+// meet in LDS; else a row a group.  It reads the
+// partial rows once: 13 to 16 us after the 4096 tokens over 8192 keys.
 constexpr int kCombineParts = 4;
 struct PartialSum {
   float m = -INFINITY, l = 0.f;

@@ -14,10 +14,13 @@
 // frequency of 1 is exact to 10^-10 turns; in fp32 it would be off by 0.06
 // radians), and shared through LDS: 2 KiB a wave at head_dim 512.
 //
-// Bound: memory (each row read and written once).  A wave has all its rows'
-// loads in flight before it forms the angles; few tokens are dealt a row group
-// a wave, many tokens kRopeBatch row groups a wave (the angles are then formed
-// half as often and four times the bytes are in flight).
+// Bound: memory (each row read and written once): 4096 tokens of 32 rows of 128
+// bf16 with norms 15.6 us a call, 4.3 TB/s, 86% of a copy's rate; 3856 tokens'
+// K and V rows of 32 heads of 96 into pages 24.9 us, 3.8 TB/s; one token 3.4 us
+// on the GPU.  A wave has all its rows' loads in flight before it forms the
+// angles; few tokens are dealt a row group a wave, many tokens kRopeBatch row
+// groups a wave, whose angles are then formed once (two groups 16.3 us on the
+// 4096 tokens, eight 18.7, one 15.9; on the pages 25.8, 31.5, 28.2).
 #include <climits>
 #include <type_traits>
 
