@@ -433,7 +433,7 @@ typedef struct {
   kiv_paged_batch_t batch;
   const void *q;           /* [total_q, Hq, D], strides t, h */
   int64_t q_stride[2];
-  void *out;               /* [total_q, Hq, D] contiguous */
+  void *out;               /* [total_q, Hq, D] contiguous; overlaps neither q (refused) nor the pages */
   int32_t num_q_heads;     /* Hq % Hkv == 0, q head h reads kv head h / (Hq / Hkv) */
   int32_t window;          /* > 0: a token sees its own key and the window - 1 before it */
   float scaling;           /* positive */

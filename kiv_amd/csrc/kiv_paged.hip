@@ -1122,6 +1122,13 @@ int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream
   if (w.total > 0 && (!a->workspace || a->workspace_bytes < w.total || ((uintptr_t)a->workspace & 255)))
     return fail(KIV_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %zu bytes "
                 "(kiv_paged_attention_workspace_size)", who, w.total);
+  // A unit's rows may be written before another block reads its own query rows.
+  const int64_t q_end[2] = {(b.total_q - 1) * a->q_stride[0] * eb, (a->num_q_heads - 1) * a->q_stride[1] * eb};
+  const int64_t row = (int64_t)c.head_dim * eb, q0 = (int64_t)(uintptr_t)a->q, o0 = (int64_t)(uintptr_t)a->out;
+  const int64_t lo = q0 + std::min<int64_t>(q_end[0], 0) + std::min<int64_t>(q_end[1], 0);
+  const int64_t hi = q0 + std::max<int64_t>(q_end[0], 0) + std::max<int64_t>(q_end[1], 0) + row;
+  if (o0 < hi && lo < o0 + (int64_t)b.total_q * a->num_q_heads * row)
+    return fail(KIV_ERR_INVALID, "%s: out must not overlap the query", who);
   PagedAttnParams p;
   p.q = (const char *)a->q;
   p.q_t = a->q_stride[0] * eb;

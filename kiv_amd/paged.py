@@ -246,8 +246,8 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
     those.  Append the new tokens first.  Query head h reads key head
     h // (Hq / Hkv); head_dim 32, 64, 96, 128, 192 or 256.
 
-    Returns [tokens, Hq, D]: ``out`` (contiguous) or a new tensor.  Rows that
-    see no key are zero; rows past the last sequence stay as they are (in a
+    Returns [tokens, Hq, D]: ``out`` (contiguous; it must overlap neither the
+    query nor the pages) or a new tensor.  Rows that see no key are zero; rows past the last sequence stay as they are (in a
     new tensor: undefined).
     """
     no_grad_check("paged_attention", query)

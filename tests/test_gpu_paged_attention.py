@@ -342,6 +342,23 @@ def test_paged_attention_refusals(cuda):
     assert paged_attention(dq[:0], cache, batch, 1.0).shape == (0, 4, 64)
 
 
+def test_out_over_the_query(cuda):
+    """Refused wherever they share memory; next to each other they may lie."""
+    g = torch.Generator().manual_seed(73)
+    cache, batch, table, cu, q, k, v = setup(g, BF16, [40, 1], [300, 77], 4, 2, 64, 16, False, cuda)
+    both = torch.zeros(82, 4, 64, dtype=BF16, device=cuda)
+    for at in (0, 1, 40):
+        with pytest.raises(RuntimeError, match="overlap"):
+            paged_attention(both[:41], cache, batch, 0.125, out=both[at:at + 41])
+    with pytest.raises(RuntimeError, match="overlap"):
+        paged_attention(both[40:81], cache, batch, 0.125, out=both[:41])
+    for lo, hi in ((0, 41), (41, 0)):
+        both[lo:lo + 41] = q.to(cuda)
+        out = paged_attention(both[lo:lo + 41], cache, batch, 0.125, out=both[hi:hi + 41])
+        assert out.data_ptr() == both[hi].data_ptr()
+        verify(out, q, k, v, table, [300, 77], cu, 0.125)
+
+
 def test_handles_keep_their_tensors(cuda):
     """The kernels read through addresses taken at construction: the tensors
     behind them cannot be swapped, and live as long as the handle."""

@@ -179,6 +179,20 @@ def test_paged_attention_refusals(code, over):
     assert b"kiv_paged_attention" in lib.kiv_last_error()
 
 
+@pytest.mark.parametrize("over", [
+    dict(),                                               # the query itself
+    dict(out=AT + 512),                                   # a token further
+    dict(out=AT + 512, q=AT + 512 * 4),                   # its last rows are the query's first
+    dict(out=AT + 512, q_stride=(C.c_int64 * 2)(512, 64)),  # between rows that lie apart
+    dict(q=AT + 512 * 8, q_stride=(C.c_int64 * 2)(-256, 64)),
+])
+def test_paged_attention_out_over_the_query(over):
+    lib = nat.lib()
+    args = attention_args(batch__total_q=5, **over)
+    assert lib.kiv_paged_attention(C.byref(args), None) == nat.ERR_INVALID
+    assert b"overlap" in lib.kiv_last_error()
+
+
 def test_paged_workspace_size():
     lib = nat.lib()
     assert lib.kiv_paged_attention_workspace_size(None) == 0
