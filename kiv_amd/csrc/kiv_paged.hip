@@ -923,13 +923,15 @@ __device__ __forceinline__ PartialSum paged_sum_parts(const PagedAttnParams &p, 
     float m = s.m;
 #pragma unroll
     for (int k = 0; k < kCombineParts; ++k) m = fmaxf(m, ms[k]);
-    if (m == -INFINITY) continue;
-    const float a = s.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s.m - m);
+    // A part without a weight (l = 0) adds nothing.  One whose scores are all
+    // NaN has m = -inf too, but l is NaN, and with any weight stays it.
+    const float a = s.l == 0.f ? 0.f : __builtin_amdgcn_exp2f(s.m - m);
     s.l *= a;
     s.o *= a;
 #pragma unroll
     for (int k = 0; k < kCombineParts; ++k) {
-      const float w = ms[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[k] - m);
+      if (ls[k] == 0.f) continue;
+      const float w = __builtin_amdgcn_exp2f(ms[k] - m);
       s.l = fmaf(w, ls[k], s.l);
       s.o += w * os[k];
     }

@@ -1,0 +1,89 @@
+"""paged_attention's numbers where a sum is cut or a type is narrow: NaN in
+queries and keys, whole and divided units alike; against references that take
+long key ranges at once."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from kiv_amd import PagedBatch, PagedKVCache, paged_attention
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+PAGE = 64
+
+
+def pool(k, v, dtype, cuda):
+    """A cache of one sequence whose pages lie in order, and its table."""
+    n, hkv, D = k.shape
+    pages = -(-n // PAGE)
+    rows = torch.zeros(2, pages * PAGE, hkv, D, dtype=dtype, device=cuda)
+    rows[0, :n], rows[1, :n] = k, v
+    cache = PagedKVCache.from_pages(*(t.view(pages, PAGE, hkv, D).transpose(1, 2) for t in rows))
+    return cache, torch.arange(pages, dtype=torch.int32, device=cuda)[None]
+
+
+def one_sequence(table, n, T, cuda, hint=True):
+    return PagedBatch(table, torch.tensor([n], dtype=torch.int32, device=cuda),
+                      torch.tensor([0, T], dtype=torch.int32, device=cuda), max_q_len=T,
+                      max_kv_len=n if hint else None)
+
+
+def reference(q, k, v, scaling):
+    """(outputs, sum of p |v|) of the last T tokens over n keys, in 64 bits
+    on the inputs' device."""
+    T, hq, D = q.shape
+    n, hkv, _ = k.shape
+    q, k, v = q.double(), k.double(), v.double()
+    hidden = torch.arange(n, device=q.device) > torch.arange(n - T, n, device=q.device)[:, None]
+    out, mag = torch.empty_like(q), torch.empty_like(q)
+    for h in range(hq):
+        g = h // (hq // hkv)
+        p = torch.softmax((q[:, h] @ k[:, g].T * scaling).masked_fill(hidden, -float("inf")), -1)
+        out[:, h], mag[:, h] = p @ v[:, g], p @ v[:, g].abs()
+    return out, mag
+
+
+# Keys of a unit that goes whole, of one that is divided, and of one cut into
+# many parts (whose merge splits them over a block).
+SHAPES = [(300, 1), (6000, 1), (90_000, 1), (300, 70), (9000, 70)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n,T", SHAPES)
+@pytest.mark.parametrize("hint", [True, False], ids=["hint", "nohint"])
+def test_nan_query_rows_are_nan(cuda, dtype, n, T, hint):
+    """A query row of NaN gives a row of NaN however its unit is cut, and no
+    other row is touched."""
+    g = torch.Generator(device=cuda).manual_seed(n + T)
+    k, v = (torch.randn(n, 2, 64, device=cuda, generator=g).to(dtype) for _ in range(2))
+    q = torch.randn(T, 8, 64, device=cuda, generator=g).to(dtype)
+    cache, table = pool(k, v, dtype, cuda)
+    batch = one_sequence(table, n, T, cuda, hint)
+    want = paged_attention(q, cache, batch, 0.125)
+    assert torch.isfinite(want).all()
+    hit = torch.zeros(T, 8, dtype=torch.bool, device=cuda)
+    hit[0, 3] = hit[T // 2, 5] = hit[T - 1, 0] = True
+    got = paged_attention(torch.where(hit[..., None], float("nan"), q), cache, batch, 0.125)
+    assert torch.isnan(got[hit]).all()
+    assert torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n,T", SHAPES)
+@pytest.mark.parametrize("first,share", [(0, 0.4), (0.3, 0.5), (0.5, 0.5)])
+def test_nan_keys_reach_the_rows_that_see_them(cuda, dtype, n, T, first, share):
+    """A range of NaN keys, longer than some of the parts a unit is cut into:
+    every row that sees one is NaN."""
+    g = torch.Generator(device=cuda).manual_seed(n + T + 1)
+    k, v = (torch.randn(n, 2, 64, device=cuda, generator=g).to(dtype) for _ in range(2))
+    q = torch.randn(T, 8, 64, device=cuda, generator=g).to(dtype)
+    a = int(first * n)
+    k[a:a + int(share * n), 1] = float("nan")
+    cache, table = pool(k, v, dtype, cuda)
+    got = paged_attention(q, cache, one_sequence(table, n, T, cuda), 0.125)
+    sees = torch.arange(n - T, n, device=cuda) >= a
+    assert torch.isnan(got[sees][:, 4:]).all()
+    assert torch.isfinite(got[:, :4]).all() and torch.isfinite(got[~sees]).all()
