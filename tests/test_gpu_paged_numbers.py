@@ -1,6 +1,6 @@
 """paged_attention's numbers where a sum is cut or a type is narrow: NaN in
-queries and keys, whole and divided units alike; against references that take
-long key ranges at once."""
+queries and keys, whole and divided units alike, and many small weights
+beside a large one; against references that take long key ranges at once."""
 
 from __future__ import annotations
 
@@ -87,3 +87,31 @@ def test_nan_keys_reach_the_rows_that_see_them(cuda, dtype, n, T, first, share):
     sees = torch.arange(n - T, n, device=cuda) >= a
     assert torch.isnan(got[sees][:, 4:]).all()
     assert torch.isfinite(got[:, :4]).all() and torch.isfinite(got[~sees]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("n,T", [(400, 1), (400, 33), (1 << 17, 1), (1 << 20, 1), (1 << 17, 33)])
+def test_many_small_weights_beside_a_large_one(cuda, dtype, n, T):
+    """One key, worth nothing, 13 to 17.5 nats above all others, each worth 64:
+    the output is the others' share, in closed form.  16-bit types round it at
+    the store and each probability as an operand, half a step each (all the
+    others' probabilities are alike, so theirs does not average out); fp32 sums
+    lose at most half a step an addition, of which a lane makes one for each 16
+    of the keys (chunks: for each 2), and the exponentials and quotients a few
+    more."""
+    gaps = torch.tensor([13.0, 14.1875, 15.5, 16.375, 17.0, 17.1875, 17.375, 17.5], dtype=torch.float64)
+    k, v = torch.zeros(2, n, 1, 64, device=cuda, dtype=dtype)
+    k[5, 0, 0] = 1.0
+    v[:] = 64.0
+    v[5] = 0.0
+    q = torch.zeros(T, len(gaps), 64, device=cuda, dtype=dtype)
+    q[:, :, 0] = gaps.to(cuda, dtype)
+    gaps = q[0, :, 0].double().cpu()
+    cache, table = pool(k, v, dtype, cuda)
+    got = paged_attention(q, cache, one_sequence(table, n, T, cuda), 1.0).double().cpu()
+    others = (torch.arange(n - T, n, dtype=torch.float64))[:, None]
+    want = (64 * others / (others + gaps.exp()))[..., None]
+    half = torch.finfo(dtype).eps / 2
+    bound = (half + (0 if dtype == F32 else half * (1 + half)) + (n / (16 if T == 1 else 2) + 64) * 2.0 ** -24) * want
+    over, off = float(((got - want).abs() - bound).max()), float(((got - want).abs() / want).max())
+    assert over <= 0, f"off by up to {off:.2g} of the value"
