@@ -402,8 +402,8 @@ typedef struct {
   const int32_t *block_table; /* [num_seqs, table_width] pages; row stride table_stride (elements) */
   int64_t table_stride;
   int32_t num_seqs, table_width, total_q; /* total_q: packed rows */
-  int32_t max_q_len, max_kv_len;          /* bounds of the lengths (they choose the kernel only: wrong ones cost
-                                             time, not results) */
+  int32_t max_q_len, max_kv_len;          /* bounds of the lengths (they choose the kernel only, and with it the
+                                             results' rounding: wrong ones cost time) */
   int32_t _pad;
 } kiv_paged_batch_t;
 
@@ -447,13 +447,14 @@ typedef struct {
 size_t kiv_paged_attention_workspace_size(const kiv_paged_attention_args_t *args);
 
 /* One softmax per packed row and head over the keys of its sequence up to its
- * own (the causal rule), in fp32; with fp16 and bf16 the probabilities are
- * rounded to the dtype before they weight V.  Rows that see no key are zero;
- * rows behind the last sequence are left as they are.  Values of keys that
- * any row of the call sees must be finite: as in a product of matrices, a NaN
- * in V reaches neighbouring rows whose weight for it is zero.  Rows past a
- * sequence's length, and of other sequences, are never read.  Two calls may
- * run at once if they have workspaces of their own. */
+ * own (the causal rule), in fp32.  With fp16 and bf16, calls of more than 16
+ * rows a kv head and sequence (by max_q_len) round the probabilities to the
+ * dtype before they weight V; the others weight by fp32's to 2^-16.  Rows that
+ * see no key are zero; rows behind the last sequence are left as they are.
+ * Values of keys that any row of the call sees must be finite: as in a product
+ * of matrices, a NaN in V reaches neighbouring rows whose weight for it is
+ * zero.  Rows past a sequence's length, and of other sequences, are never
+ * read.  Two calls may run at once if they have workspaces of their own. */
 int kiv_paged_attention(const kiv_paged_attention_args_t *args, kiv_stream_t stream);
 
 #ifdef __cplusplus

@@ -91,8 +91,8 @@ class PagedBatch:
                  of the last; rows past it are no sequence's.  None: one new
                  token a sequence.
     max_q_len, max_kv_len  bounds of the lengths, known to the host; they
-                 choose the kernel only (a wrong one costs time, not results).
-                 Defaults: no bound.
+                 choose the kernel only, and with it the results' rounding
+                 (a wrong one costs time).  Defaults: no bound.
 
     The arrays stay the caller's: update them in place between steps (or
     between replays of a captured graph).
@@ -244,7 +244,9 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
     over the keys of their sequences, up to each token's own
     (kv_len[b] - cu_q[b + 1] + row); with ``window`` the last ``window`` of
     those.  Append the new tokens first.  Query head h reads key head
-    h // (Hq / Hkv); head_dim 32, 64, 96, 128, 192 or 256.
+    h // (Hq / Hkv); head_dim 32, 64, 96, 128, 192 or 256.  fp32 inside; fp16
+    and bf16 batches of more than 16 rows a key head and sequence (by the
+    batch's max_q_len) weight V by probabilities rounded to the dtype.
 
     Returns [tokens, Hq, D]: ``out`` (contiguous; it must overlap neither the
     query nor the pages) or a new tensor.  Rows that see no key are zero; rows past the last sequence stay as they are (in a

@@ -1,6 +1,7 @@
 """paged_attention's numbers where a sum is cut or a type is narrow: NaN in
-queries and keys, whole and divided units alike, and many small weights
-beside a large one; against references that take long key ranges at once."""
+queries and keys, whole and divided units alike, many small weights beside a
+large one, and weights that 16 bits do not hold; against references that take
+long key ranges at once."""
 
 from __future__ import annotations
 
@@ -115,3 +116,25 @@ def test_many_small_weights_beside_a_large_one(cuda, dtype, n, T):
     bound = (half + (0 if dtype == F32 else half * (1 + half)) + (n / (16 if T == 1 else 2) + 64) * 2.0 ** -24) * want
     over, off = float(((got - want).abs() - bound).max()), float(((got - want).abs() / want).max())
     assert over <= 0, f"off by up to {off:.2g} of the value"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("n,T", [(37, 1), (700, 4), (9000, 1)])
+def test_tokens_weigh_values_by_more_than_16_bits(cuda, dtype, D, n, T):
+    """Units of 16 rows hold a probability to 2^-16 (fp16 2^-22 and, far under
+    the maximum, 2^-36) of its value.  Scores are exact products here, so that
+    fp32 adds only their scaling's and exponentials' half steps and one an
+    addition (a lane adds one in 16 of the keys)."""
+    g = torch.Generator(device=cuda).manual_seed(D + n)
+    k, v = (torch.randn(n, 2, D, device=cuda, generator=g).to(dtype) for _ in range(2))
+    q = torch.zeros(T, 8, D, device=cuda, dtype=dtype)
+    q[:, :, 0] = torch.rand(T, 8, device=cuda, generator=g) * 3
+    cache, table = pool(k, v, dtype, cuda)
+    got = paged_attention(q, cache, one_sequence(table, n, T, cuda), 1.0).double()
+    ref, mag = reference(q, k, v, 1.0)
+    top = float(q.abs().max() * k[:, :, 0].abs().max())
+    rest, gone = (2.0 ** -16, 0.0) if dtype == BF16 else (2.0 ** -22, n * 2.0 ** -36 * float(v.abs().max()) + 2.0 ** -25)
+    bound = torch.finfo(dtype).eps / 2 * ref.abs() + (rest + (8 * top + n / 16 + 64) * 2.0 ** -24) * mag + gone
+    over = float(((got - ref).abs() - bound).max())
+    assert over <= 0, f"{over:.2g} over the bound"
