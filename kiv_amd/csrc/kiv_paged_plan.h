@@ -28,8 +28,9 @@ struct FastDiv {
   KIV_HD int div(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
 };
 
-// A sequence as the kernels take it: its packed rows [q0, q0 + qlen) and its
-// length, brought into range whatever the arrays hold.
+// A sequence as the kernels take it: its packed rows [q0, q0 + qlen), brought
+// into range whatever the arrays hold, and its keys up to the last of those
+// (the whole length, less the rows behind the call's; then maybe negative).
 struct PagedSeq {
   int q0, qlen, len;
 };
@@ -71,7 +72,9 @@ struct PagedShape {
     q.q0 = cu0 < 0 ? 0 : cu0 > total_q ? total_q : cu0;
     const int end = cu1 < 0 ? 0 : cu1 > total_q ? total_q : cu1;
     q.qlen = end > q.q0 ? end - q.q0 : 0;
-    q.len = len < 0 ? 0 : len;
+    // Row r has key kv_len - cu_q[b + 1] + r; a negative length has no keys, as
+    // a length of 0.
+    q.len = (len < 0 ? 0 : len) - (q.qlen > 0 ? cu1 - end : 0);
     return q;
   }
   // Units of one kv head of a sequence.

@@ -8,7 +8,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from kiv_amd import PagedBatch, PagedKVCache, paged_attention
+from kiv_amd import PagedBatch, PagedKVCache, paged_append, paged_attention
+from tests.paged_ref import attention_bound, check
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +139,19 @@ def test_tokens_weigh_values_by_more_than_16_bits(cuda, dtype, D, n, T):
     bound = torch.finfo(dtype).eps / 2 * ref.abs() + (rest + (8 * top + n / 16 + 64) * 2.0 ** -24) * mag + gone
     over = float(((got - ref).abs() - bound).max())
     assert over <= 0, f"{over:.2g} over the bound"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n,T,rows", [(300, 90, 41), (300, 4, 1), (5000, 64, 30)])
+def test_a_prefix_of_a_steps_rows(cuda, dtype, n, T, rows):
+    """cu_q runs past the rows that a call is given: append and attention
+    give each row the key that it has in the whole step."""
+    g = torch.Generator(device=cuda).manual_seed(n + T)
+    k, v = (torch.randn(n, 2, 64, device=cuda, generator=g).to(dtype) for _ in range(2))
+    q = torch.randn(T, 8, 64, device=cuda, generator=g).to(dtype)
+    cache, table = pool(k * (torch.arange(n, device=cuda) < n - T)[:, None, None], v, dtype, cuda)
+    whole = one_sequence(table, n, T, cuda)
+    paged_append(cache, whole, k[n - T:][:rows], v[n - T:][:rows])
+    got = paged_attention(q[:rows], cache, whole, 0.125)
+    ref, mag = (x[:rows].cpu() for x in reference(q, k, v, 0.125))
+    check(got, ref, attention_bound(ref, mag, q.cpu(), k.cpu(), dtype, 0.125, n))

@@ -159,3 +159,52 @@ def test_units_shares_and_quotients(tmp_path):
                     str(tmp_path / "walk.cpp"), "-o", str(tmp_path / "walk")], check=True)
     res = subprocess.run([str(tmp_path / "walk")], capture_output=True, text=True, timeout=120)
     assert res.returncode == 0 and res.stdout.strip() == "0", res.stdout + res.stderr
+
+
+KEYS = r"""
+#include <stdio.h>
+#include <algorithm>
+#include <random>
+#include "%s"
+using namespace kiv;
+
+// The key index of packed row r of a sequence is kv_len - cu_q[b + 1] + r,
+// also where cu_q leaves the rows that the call has.
+int main() {
+  std::mt19937 g(3);
+  auto pick = [&](int lo, int hi) { return lo + (int)(g() %% (unsigned)(hi - lo + 1)); };
+  long long bad = 0, rows = 0;
+  for (int i = 0; i < 20000; ++i) {
+    const int total_q = pick(0, 60), page = pick(1, 30), cap = page * pick(0, 30), G = pick(1, 20);
+    const PagedShape sh = PagedShape::of(total_q, 1, G, pick(0, 1) ? 16 : 128, cap, 6, 0, false, 1);
+    const int cu0 = pick(-20, 70), far = pick(0, 4);
+    const int cu1 = far == 0 ? 2147483647 : far == 1 ? cu0 + pick(-5, 200) : cu0 + pick(0, 40);
+    const int len = pick(0, 9) ? pick(0, 300) : pick(0, 1) ? 2147483647 : -pick(1, 2147483647);
+    const PagedSeq s = sh.seq(cu0, cu1, len);
+    for (int rt = 0; rt < sh.row_tiles(s); ++rt) {
+      int k0, k1;
+      sh.keys(s, rt, k0, k1);
+      const int tok0 = sh.token0(rt), last = tok0 + sh.tokens(s, tok0) - 1;
+      const long long key = (long long)len - cu1 + s.q0 + last;
+      const long long want = std::max(0LL, std::min<long long>(cap, key + 1));
+      ++rows;
+      if (k0 != 0 || k1 != want) {
+        if (bad++ < 5) printf("rows %%d cu %%d %%d len %%d: keys to %%d, not %%lld\n", total_q, cu0, cu1, len, k1, want);
+      }
+    }
+  }
+  printf("%%lld of %%lld\n", bad, rows);
+  return bad != 0 || rows < 10000;
+}
+"""
+
+
+def test_keys_where_cu_q_leaves_the_rows(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    (tmp_path / "keys.cpp").write_text(KEYS % HEADER)
+    subprocess.run([gxx, "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=all",
+                    str(tmp_path / "keys.cpp"), "-o", str(tmp_path / "keys")], check=True)
+    res = subprocess.run([str(tmp_path / "keys")], capture_output=True, text=True, timeout=120)
+    assert res.returncode == 0, res.stdout + res.stderr
