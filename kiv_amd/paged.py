@@ -166,7 +166,7 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
     are left alone, in the pages and in ``q_out``; a token whose page is not
     there is dropped.
     """
-    no_grad_check("paged_append", q, k, v)
+    no_grad_check("paged_append", q, k, v, cache._k, cache._v, rotary, q_norm, k_norm, v_norm, q_out)
     key = (cache._geometry, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype,
            None if q is None else (q.shape, q.stride(), q.dtype))
     plan = _append_plans.get(key)
@@ -252,7 +252,7 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
     query nor the pages) or a new tensor.  Rows that see no key are zero; rows past the last sequence stay as they are (in a
     new tensor: undefined).
     """
-    no_grad_check("paged_attention", query)
+    no_grad_check("paged_attention", query, cache._k, cache._v, out)
     dev = cache.device
     if query.device != dev or batch.device != dev:
         raise ValueError(f"query is on {query.device}, the batch on {batch.device}, the cache on {dev}")

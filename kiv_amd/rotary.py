@@ -11,6 +11,7 @@ No counterpart in the reference, whose models run their own rotation.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -19,10 +20,14 @@ class HeadNorm:
     """Norm of each head's row: ``x / sqrt(mean(x^2) + eps) * (weight + offset)``.
 
     ``weight`` ([head_dim], or None for a norm without a scale) is copied in
-    fp32 at construction; build another object after changing it.
+    fp32 at construction; build another object after changing it.  It gets no
+    gradient: one that requires it makes calls fail where gradients are
+    recorded.
     """
 
     def __init__(self, weight: torch.Tensor | None = None, eps: float = 1e-6, offset: float = 0.0) -> None:
+        no_tangent_check("HeadNorm", weight)
+        self.requires_grad = weight is not None and weight.requires_grad
         if weight is not None:
             if weight.dim() != 1:
                 raise ValueError(f"norm weight must be [head_dim], got {tuple(weight.shape)}")
@@ -56,7 +61,8 @@ class Rotary:
 
     inv_freq     [rot_dim / 2] fp32: pair i turns by position * inv_freq[i];
                  the angle is formed in 64 bits, so far positions keep the
-                 precision of near ones.
+                 precision of near ones.  It gets no gradient: one that
+                 requires it makes calls fail where gradients are recorded.
     interleaved  pairs are neighbours (2 i, 2 i + 1) instead of entries
                  rot_dim / 2 apart.
     scale        factor of the cosines and sines.
@@ -80,6 +86,8 @@ class Rotary:
             if axes.is_floating_point() or axes.dtype == torch.bool:
                 raise TypeError(f"axes must be integers, not {axes.dtype}")
             axes = axes.to(torch.int32).contiguous()
+        no_tangent_check("Rotary", inv_freq)
+        self.requires_grad = inv_freq.requires_grad
         self._inv_freq = inv_freq.detach().contiguous()
         self._axes = axes
         self.rot_dim = 2 * inv_freq.shape[0]
@@ -137,12 +145,23 @@ def _position_layout(shape, st, dtype, lead: bool, batched: bool, batch: int, to
     return nat._I64x3(sa, sb, stt), 8 if dtype == torch.int64 else 4, axes
 
 
-def no_grad_check(what: str, *tensors: torch.Tensor | None) -> None:
-    """These kernels have no backward pass: refuse to drop a gradient."""
+def no_grad_check(what: str, *inputs: torch.Tensor | HeadNorm | Rotary | None) -> None:
+    """These kernels have no derivatives: refuse to drop one, of what a call
+    reads or of what it writes over."""
     if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
+        for x in inputs:
+            if x is not None and x.requires_grad:
                 raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
+    no_tangent_check(what, *inputs)
+
+
+def no_tangent_check(what: str, *inputs: torch.Tensor | HeadNorm | Rotary | None) -> None:
+    # Tangents exist within a level only; asking each tensor costs 0.3 us.
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    for x in inputs:
+        if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 def aligned_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, nat.Layout]:
@@ -178,7 +197,7 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor |
     fp32, fp16 and bf16; head_dim a multiple of 16 bytes up to 512, the
     rotated width of 32 bytes.  Returns (q_out, k_out).
     """
-    no_grad_check("norm_rope", q, k)
+    no_grad_check("norm_rope", q, k, rotary, q_norm, k_norm, q_out, k_out)
     dev = q.device
     if dev.type != "cuda":
         raise ValueError("norm_rope needs GPU tensors")
