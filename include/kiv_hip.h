@@ -367,7 +367,10 @@ typedef struct {
 } kiv_head_norm_t;
 
 /* Rows of q and k: [B, H, T, D], strides b, h, t in elements, 16-byte aligned.
- * Outputs may be the inputs themselves (same pointer and strides). */
+ * Outputs may be the inputs themselves (same pointer and strides); other
+ * overlaps of what is written with anything that is read or written are
+ * refused (also where only the ranges of addresses meet, unless the strides
+ * agree, as of slices of one buffer). */
 typedef struct {
   int32_t batch, tokens, num_q_heads, num_kv_heads, head_dim, dtype;
   const void *q;
@@ -424,8 +427,9 @@ typedef struct {
 } kiv_paged_append_args_t;
 
 /* Writes the new tokens' K (normed, rotated) and V (normed) rows to their
- * pages, and q beside them.  Pages named twice by the table get the rows of
- * one of their sequences. */
+ * pages, and q beside them.  A slot that two new tokens name (a page that the
+ * table names twice) holds parts of both rows afterwards.  q_out may be q; the
+ * pages and q_out overlap nothing else (refused, as by kiv_norm_rope). */
 int kiv_paged_append(const kiv_paged_append_args_t *args, kiv_stream_t stream);
 
 typedef struct {
@@ -433,7 +437,7 @@ typedef struct {
   kiv_paged_batch_t batch;
   const void *q;           /* [total_q, Hq, D], strides t, h */
   int64_t q_stride[2];
-  void *out;               /* [total_q, Hq, D] contiguous; overlaps neither q (refused) nor the pages */
+  void *out;               /* [total_q, Hq, D] contiguous; overlaps neither q nor the pages (refused) */
   int32_t num_q_heads;     /* Hq % Hkv == 0, q head h reads kv head h / (Hq / Hkv) */
   int32_t window;          /* > 0: a token sees its own key and the window - 1 before it */
   float scaling;           /* positive */

@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "../../include/kiv_hip.h"
+#include "kiv_rows.h"
 
 namespace kiv {
 
@@ -48,6 +49,8 @@ struct DevBuf {
 // Argument checks of the paged cache's entry points (host only).
 int paged_cache_check(const kiv_paged_cache_t &c, const char *who);
 int paged_batch_check(const kiv_paged_batch_t &b, const kiv_paged_cache_t &c, const char *who);
+// The rows of the pages at `pages` (the cache's K or V).
+RowSet page_rows(const kiv_paged_cache_t &c, const void *pages);
 
 inline int elem_bytes(int dtype) { return dtype == KIV_DTYPE_F32 ? 4 : 2; }
 inline int vec_elems(int dtype) { return 16 / elem_bytes(dtype); }

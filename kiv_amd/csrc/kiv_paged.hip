@@ -1163,6 +1163,9 @@ int kiv_paged_attention(const kiv_paged_attention_args_t *a, kiv_stream_t stream
   const int64_t hi = q0 + std::max<int64_t>(q_end[0], 0) + std::max<int64_t>(q_end[1], 0) + row;
   if (o0 < hi && lo < o0 + (int64_t)b.total_q * a->num_q_heads * row)
     return fail(KIV_ERR_INVALID, "%s: out must not overlap the query", who);
+  const RowSet out = {a->out, {0, a->num_q_heads * row, row}, {1, b.total_q, a->num_q_heads}, row};
+  if (rows_overlap(out, page_rows(c, c.k)) || rows_overlap(out, page_rows(c, c.v)))
+    return fail(KIV_ERR_INVALID, "%s: out must not overlap the pages", who);
   PagedAttnParams p;
   p.q = (const char *)a->q;
   p.q_t = a->q_stride[0] * eb;

@@ -256,6 +256,23 @@ static int aligned_check(const char *who, const void *p, const int64_t *stride, 
   return KIV_OK;
 }
 
+// Rows that are written: apart from each other, and from rows that other
+// waves read or write, or the bytes depend on which wave comes first.
+static int written_check(const char *who, const char *name, const RowSet &rows) {
+  if (rows_fold(rows)) return fail(KIV_ERR_INVALID, "%s: rows of %s share memory", who, name);
+  return KIV_OK;
+}
+static int apart_check(const char *who, const char *name, const RowSet &a, const char *other, const RowSet &b) {
+  if (rows_overlap(a, b)) return fail(KIV_ERR_INVALID, "%s: %s must not overlap %s", who, name, other);
+  return KIV_OK;
+}
+// An output may be its input: a wave has read a row before it writes it.
+static int in_place_check(const char *who, const char *name, const RowSet &out, const char *input, const RowSet &in) {
+  if (!rows_same(out, in) && rows_overlap(out, in))
+    return fail(KIV_ERR_INVALID, "%s: %s must be %s or not overlap it", who, name, input);
+  return KIV_OK;
+}
+
 static void fill_rotary(RopeParams &p, const kiv_rotary_t &r, int dtype) {
   p.half = r.rot_dim / (2 * vec_elems(dtype));
   p.inv_freq = r.inv_freq;
@@ -344,6 +361,12 @@ int paged_cache_check(const kiv_paged_cache_t &c, const char *who) {
   return rc ? rc : aligned_check(who, c.v, c.stride, 3, c.dtype);
 }
 
+RowSet page_rows(const kiv_paged_cache_t &c, const void *pages) {
+  const int64_t eb = elem_bytes(c.dtype);
+  return {pages, {c.stride[0] * eb, c.stride[2] * eb, c.stride[1] * eb}, {c.num_pages, c.page_size, c.num_kv_heads},
+          c.head_dim * eb};
+}
+
 int paged_batch_check(const kiv_paged_batch_t &b, const kiv_paged_cache_t &c, const char *who) {
   if (b.num_seqs < 0 || b.table_width < 0 || b.total_q < 0)
     return fail(KIV_ERR_INVALID, "%s: negative batch sizes", who);
@@ -378,8 +401,20 @@ int kiv_norm_rope(const kiv_norm_rope_args_t *a, kiv_stream_t stream) {
   if (a->num_kv_heads > 0 && ((rc = aligned_check(who, a->k, a->k_stride, 3, a->dtype)) ||
                               (rc = aligned_check(who, a->k_out, a->k_out_stride, 3, a->dtype))))
     return rc;
-  RopeParams p = {};
   const int eb = elem_bytes(a->dtype);
+  auto rows = [&](const void *at, const int64_t *stride, int heads) {
+    return RowSet{at, {stride[0] * eb, stride[1] * eb, stride[2] * eb}, {a->batch, heads, a->tokens},
+                  (int64_t)a->head_dim * eb};
+  };
+  const RowSet q = rows(a->q, a->q_stride, a->num_q_heads), k = rows(a->k, a->k_stride, a->num_kv_heads);
+  const RowSet q_out = rows(a->q_out, a->q_out_stride, a->num_q_heads);
+  const RowSet k_out = rows(a->k_out, a->k_out_stride, a->num_kv_heads);
+  if ((rc = written_check(who, "q_out", q_out)) || (rc = written_check(who, "k_out", k_out)) ||
+      (rc = in_place_check(who, "q_out", q_out, "q", q)) || (rc = in_place_check(who, "k_out", k_out, "k", k)) ||
+      (rc = apart_check(who, "q_out", q_out, "k", k)) || (rc = apart_check(who, "k_out", k_out, "q", q)) ||
+      (rc = apart_check(who, "q_out", q_out, "k_out", k_out)))
+    return rc;
+  RopeParams p = {};
   p.q = rope_rows(a->q, a->q_stride[0], a->q_stride[1], a->q_stride[2], a->q_out, a->q_out_stride[0],
                   a->q_out_stride[1], a->q_out_stride[2], a->q_norm, a->num_q_heads, eb);
   p.k = rope_rows(a->k, a->k_stride[0], a->k_stride[1], a->k_stride[2], a->k_out, a->k_out_stride[0],
@@ -407,8 +442,23 @@ int kiv_paged_append(const kiv_paged_append_args_t *a, kiv_stream_t stream) {
   if (a->num_q_heads > 0 && ((rc = aligned_check(who, a->q, a->q_stride, 2, c.dtype)) ||
                              (rc = aligned_check(who, a->q_out, a->q_out_stride, 2, c.dtype))))
     return rc;
-  RopeParams p = {};
   const int eb = elem_bytes(c.dtype);
+  auto rows = [&](const void *at, const int64_t *stride, int heads) {  // axes as page_rows has them
+    return RowSet{at, {0, stride[0] * eb, stride[1] * eb}, {1, b.total_q, heads}, (int64_t)c.head_dim * eb};
+  };
+  const RowSet k_pages = page_rows(c, c.k), v_pages = page_rows(c, c.v);
+  const RowSet k = rows(a->k, a->k_stride, c.num_kv_heads), v = rows(a->v, a->v_stride, c.num_kv_heads);
+  const RowSet q = rows(a->q, a->q_stride, a->num_q_heads), q_out = rows(a->q_out, a->q_out_stride, a->num_q_heads);
+  if ((rc = written_check(who, "the pages", k_pages)) || (rc = apart_check(who, "K pages", k_pages, "V pages", v_pages)))
+    return rc;
+  for (const RowSet &pages : {k_pages, v_pages})
+    if ((rc = apart_check(who, "the pages", pages, "k", k)) || (rc = apart_check(who, "the pages", pages, "v", v)) ||
+        (rc = apart_check(who, "the pages", pages, "q", q)) || (rc = apart_check(who, "the pages", pages, "q_out", q_out)))
+      return rc;
+  if ((rc = written_check(who, "q_out", q_out)) || (rc = in_place_check(who, "q_out", q_out, "q", q)) ||
+      (rc = apart_check(who, "q_out", q_out, "k", k)) || (rc = apart_check(who, "q_out", q_out, "v", v)))
+    return rc;
+  RopeParams p = {};
   p.q = rope_rows(a->q, 0, a->q_stride[1], a->q_stride[0], a->q_out, 0, a->q_out_stride[1], a->q_out_stride[0],
                   a->q_norm, a->num_q_heads, eb);
   p.k = rope_rows(a->k, 0, a->k_stride[1], a->k_stride[0], c.k, c.stride[0], c.stride[1], c.stride[2], a->k_norm,

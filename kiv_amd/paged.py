@@ -161,10 +161,11 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
     [tokens] or, with ``rotary.axes``, [axes, tokens]; None turns each token
     by its key index.  With q [tokens, Hq, D] the queries are normed
     (``q_norm``) and turned in the same launch, into ``q_out`` (new by
-    default; may be q, and must not overlap it otherwise); returns it, else
-    None.  Rows past the last sequence
-    are left alone, in the pages and in ``q_out``; a token whose page is not
-    there is dropped.
+    default; may be q itself); returns it, else None.  Any other overlap of the
+    pages or ``q_out`` with each other or the inputs is refused.  Rows past the
+    last sequence are left alone, in the pages and in ``q_out``; a token whose
+    page is not there is dropped; a slot that two new tokens name holds parts
+    of both rows.
     """
     no_grad_check("paged_append", q, k, v, cache._k, cache._v, rotary, q_norm, k_norm, v_norm, q_out)
     key = (cache._geometry, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype,
@@ -248,9 +249,9 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
     and bf16 batches of more than 16 rows a key head and sequence (by the
     batch's max_q_len) weight V by probabilities rounded to the dtype.
 
-    Returns [tokens, Hq, D]: ``out`` (contiguous; it must overlap neither the
-    query nor the pages) or a new tensor.  Rows that see no key are zero; rows past the last sequence stay as they are (in a
-    new tensor: undefined).
+    Returns [tokens, Hq, D]: ``out`` (contiguous; refused if it overlaps the
+    query or the pages) or a new tensor.  Rows that see no key are zero; rows
+    past the last sequence stay as they are (in a new tensor: undefined).
     """
     no_grad_check("paged_attention", query, cache._k, cache._v, out)
     dev = cache.device

@@ -192,8 +192,8 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor |
 
     positions: [T], [B, T] or, with ``rotary.axes``, [axes, T] or
     [axes, B, T]; int32 or int64.  ``q_out`` / ``k_out`` may be the inputs
-    themselves (and must not overlap them otherwise); by default they are new
-    tensors in the inputs' memory order.
+    themselves (any other overlap of theirs is refused); by default they are
+    new tensors in the inputs' memory order.
     fp32, fp16 and bf16; head_dim a multiple of 16 bytes up to 512, the
     rotated width of 32 bytes.  Returns (q_out, k_out).
     """
