@@ -158,7 +158,10 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(RopeParams p) {
     unpack_chunk<DT>(x1[u], z);
     float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) ss = fmaf(in0 ? a[j] : 0.f, a[j], fmaf(in1 ? z[j] : 0.f, z[j], ss));
+    for (int j = 0; j < VEC; ++j) {  // lanes past the row hold its first chunk: an infinity there times 0 is NaN
+      const float x = in0 ? a[j] : 0.f, y = in1 ? z[j] : 0.f;
+      ss = fmaf(x, x, fmaf(y, y, ss));
+    }
     ss = group_sum<LPR>(ss);  // every lane of the wave is here
     if (s.norm) {
       const float inv = rsqrtf(fmaf(ss, p.inv_dim, s.eps));

@@ -310,3 +310,16 @@ def test_paged_refusals(cuda):
     paged_append(cache, batch, k, k)
     none = PagedBatch(table[:0], lens[:0])
     assert paged_append(cache, none, k[:0], k[:0]) is None
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 96), (F16, 40), (F32, 20), (BF16, 128), (F16, 8)])
+@pytest.mark.parametrize("at", [0, 7])
+def test_an_infinity_hides_only_itself(cuda, dtype, D, at):
+    """A row with an infinity has an infinite mean: its other entries become
+    0, itself NaN, at widths whose lanes do not all hold a chunk too."""
+    x = torch.randn(1, 2, 3, D, device=cuda).to(dtype)
+    x[0, 1, 2, at] = float("inf")
+    got, _ = norm_rope(x, None, None, None, HeadNorm())
+    row = got[0, 1, 2]
+    assert torch.isnan(row[at]) and (row[torch.arange(D, device=cuda) != at] == 0).all()
+    assert torch.isfinite(got[0, 0]).all() and torch.isfinite(got[0, 1, :2]).all()
