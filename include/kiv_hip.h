@@ -440,7 +440,7 @@ typedef struct {
   void *out;               /* [total_q, Hq, D] contiguous; overlaps neither q nor the pages (refused) */
   int32_t num_q_heads;     /* Hq % Hkv == 0, q head h reads kv head h / (Hq / Hkv) */
   int32_t window;          /* > 0: a token sees its own key and the window - 1 before it */
-  float scaling;           /* positive */
+  float scaling;           /* positive, at most 2.3e38 */
   int32_t _pad;
   void *workspace;         /* 256-byte aligned device scratch, fully rewritten by every call */
   size_t workspace_bytes;

@@ -1109,9 +1109,10 @@ static int paged_attention_check(const kiv_paged_attention_args_t *a, const char
   if (a->window < 0) return fail(KIV_ERR_INVALID, "%s: negative window", who);
   if ((int64_t)a->batch.table_width * c.page_size > (1 << 30))
     return fail(KIV_ERR_UNSUPPORTED, "%s: the block table spans over 2^30 keys", who);
-  // Hidden scores are -inf behind the scale, and the maximum is taken there.
-  if (!(a->scaling > 0.f) || !(a->scaling < INFINITY))
-    return fail(KIV_ERR_UNSUPPORTED, "%s: scaling must be positive and finite", who);
+  // Hidden scores are -inf behind the scale, and the maximum is taken there:
+  // in base 2, so the scale must be finite there too.
+  if (!(a->scaling > 0.f) || !(a->scaling * kPgLog2e < INFINITY))
+    return fail(KIV_ERR_UNSUPPORTED, "%s: scaling must be positive and finite (at most 2.3e38)", who);
   return KIV_OK;
 }
 

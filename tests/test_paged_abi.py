@@ -216,3 +216,10 @@ def test_cpu_tensors_are_refused():
         HeadNorm(torch.ones(64))
     with pytest.raises(ValueError):
         PagedKVCache(2, 8, 1, 64, device="cpu")
+
+
+@pytest.mark.parametrize("scaling", [2.4e38, 3.4e38])
+def test_scaling_that_overflows_in_base_2_is_refused(scaling):
+    lib = nat.lib()
+    assert lib.kiv_paged_attention(C.byref(attention_args(scaling=scaling)), None) == nat.ERR_UNSUPPORTED
+    assert b"scaling" in lib.kiv_last_error()
