@@ -265,6 +265,12 @@ class Layout:
         self.chunked = st[-1] == 1 and all(x % vec == 0 for x in lead)
 
 
+def check_sizes(what: str, *sizes: int) -> None:
+    """Sizes go to the library in 32 bits, which ctypes would cut silently."""
+    if max(sizes) >= 2**31:
+        raise ValueError(f"{what}: sizes of 2^31 and more are not supported, got {sizes}")
+
+
 _layouts: dict[tuple, Layout] = {}
 
 

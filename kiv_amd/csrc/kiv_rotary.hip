@@ -32,6 +32,7 @@ namespace kiv {
 constexpr int kRopeThreads = 256;
 constexpr int kRopeBatch = 4;       // row groups of a wave where there are many tokens
 constexpr int kRopeMaxDim = 512;
+constexpr int kRopeMaxHeads = 1 << 30;  // of all kinds: rows are counted in 32 bits
 constexpr int kRopeFewWaves = 4096;  // waves up to which a wave takes one row group
 
 // Rows of one kind (q, k or v): byte strides.
@@ -393,6 +394,8 @@ int kiv_norm_rope(const kiv_norm_rope_args_t *a, kiv_stream_t stream) {
   if (rc) return rc;
   if (a->batch < 0 || a->tokens < 0 || a->num_q_heads < 1 || a->num_kv_heads < 0)
     return fail(KIV_ERR_INVALID, "%s: bad sizes", who);
+  if ((int64_t)a->num_q_heads + a->num_kv_heads > kRopeMaxHeads)
+    return fail(KIV_ERR_UNSUPPORTED, "%s: over 2^30 heads", who);
   const bool none = a->batch == 0 || a->tokens == 0;
   if ((rc = rotary_check(a->rotary, a->head_dim, a->dtype, false, none, who)) || (rc = norm_check(a->q_norm, who)) ||
       (rc = norm_check(a->k_norm, who)))
@@ -438,6 +441,8 @@ int kiv_paged_append(const kiv_paged_append_args_t *a, kiv_stream_t stream) {
       (rc = norm_check(a->k_norm, who)) || (rc = norm_check(a->v_norm, who)))
     return rc;
   if (a->num_q_heads < 0) return fail(KIV_ERR_INVALID, "%s: bad sizes", who);
+  if ((int64_t)a->num_q_heads + 2 * (int64_t)c.num_kv_heads > kRopeMaxHeads)
+    return fail(KIV_ERR_UNSUPPORTED, "%s: over 2^30 heads", who);
   if (b.total_q == 0 || b.num_seqs == 0) return KIV_OK;
   if ((rc = aligned_check(who, a->k, a->k_stride, 2, c.dtype)) ||
       (rc = aligned_check(who, a->v, a->v_stride, 2, c.dtype)))

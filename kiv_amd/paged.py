@@ -55,6 +55,7 @@ class PagedKVCache:
             raise ValueError("K and V pages must be equal [num_pages, num_kv_heads, page_size, head_dim] tensors")
         if min(k.shape) < 1:
             raise ValueError(f"empty pages {tuple(k.shape)}")
+        nat.check_sizes("PagedKVCache", *k.shape)
         if k.stride() != v.stride():
             raise ValueError("K and V pages must have the same strides")
         if not k.is_cuda:
@@ -106,6 +107,7 @@ class PagedBatch:
             if n is not None and n < 0:
                 raise ValueError(f"{name} must not be negative, got {n}")
         S, W = block_table.shape
+        nat.check_sizes("PagedBatch", S, W)
         if cu_q is None:
             cu_q = torch.arange(S + 1, dtype=torch.int32, device=block_table.device)
             max_q_len = 1
@@ -144,6 +146,7 @@ def _packed_layout(t: torch.Tensor, name: str, cache: PagedKVCache, heads: int |
     shape = t.shape
     if len(shape) != 3 or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
         raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {cache.head_dim}], got {tuple(shape)}")
+    nat.check_sizes(name, *shape)
     if t.dtype != cache.dtype:
         raise TypeError(f"{name} is {t.dtype}, the cache {cache.dtype}")
     return nat.layout(t)

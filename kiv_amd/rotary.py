@@ -255,6 +255,7 @@ def _plan(q: torch.Tensor, k: torch.Tensor | None) -> tuple:
     addresses, B, T, D, q must be copied, k must be copied)."""
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("q and k must be [B, H, T, D]")
+    nat.check_sizes("norm_rope", *q.shape, *(() if k is None else k.shape))
     B, hq, T, D = q.shape
     if k is not None and ((k.shape[0], k.shape[2], k.shape[3]) != (B, T, D) or k.dtype != q.dtype):
         raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")

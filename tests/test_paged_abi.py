@@ -223,3 +223,39 @@ def test_scaling_that_overflows_in_base_2_is_refused(scaling):
     lib = nat.lib()
     assert lib.kiv_paged_attention(C.byref(attention_args(scaling=scaling)), None) == nat.ERR_UNSUPPORTED
     assert b"scaling" in lib.kiv_last_error()
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Before they are cut to 32 bits; on shapes without memory."""
+    from types import SimpleNamespace
+
+    from kiv_amd import PagedBatch, PagedKVCache, paged, rotary
+
+    def meta(*shape, dtype=torch.bfloat16):
+        return torch.empty(shape, device="meta", dtype=dtype)
+
+    n = 2**32 + 1
+    cache = SimpleNamespace(head_dim=64, num_kv_heads=1, dtype=torch.bfloat16)
+    one = meta(1, 1, 64)
+    for f in (
+        lambda: rotary._plan(meta(1, 1, n, 8), None),
+        lambda: rotary._plan(meta(1, n, 1, 8), meta(1, 1, 1, 8)),
+        lambda: rotary._plan(meta(1, 1, 1, 8), meta(1, n, 1, 8)),
+        lambda: PagedKVCache.from_pages(meta(n, 1, 1, 8), meta(n, 1, 1, 8)),
+        lambda: PagedBatch(meta(n, 1, dtype=torch.int32), meta(n, dtype=torch.int32)),
+        lambda: PagedBatch(meta(1, n, dtype=torch.int32), meta(1, dtype=torch.int32)),
+        lambda: paged._append_plan(cache, meta(n, 1, 64), meta(n, 1, 64), None),
+        lambda: paged._append_plan(cache, one, one, meta(1, n, 64)),
+        lambda: paged._attention_plan(meta(n, 1, 64), cache, None, 0),
+    ):
+        with pytest.raises(ValueError, match="2\\^31"):
+            f()
+    rotary._plan(meta(1, 1, 2**31 - 1, 8), None)
+
+
+def test_heads_past_32_bits_are_refused():
+    lib = nat.lib()
+    assert lib.kiv_norm_rope(C.byref(rope_args(num_q_heads=2**31 - 1)), None) == nat.ERR_UNSUPPORTED
+    assert lib.kiv_norm_rope(C.byref(rope_args(num_q_heads=2**30, num_kv_heads=2**30)), None) == nat.ERR_UNSUPPORTED
+    assert lib.kiv_paged_append(C.byref(append_args(num_q_heads=2**31 - 1)), None) == nat.ERR_UNSUPPORTED
+    assert lib.kiv_paged_append(C.byref(append_args(cache__num_kv_heads=2**30)), None) == nat.ERR_UNSUPPORTED
