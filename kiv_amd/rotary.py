@@ -85,6 +85,8 @@ class Rotary:
                 raise ValueError("axes must have inv_freq's shape and device")
             if axes.is_floating_point() or axes.dtype == torch.bool:
                 raise TypeError(f"axes must be integers, not {axes.dtype}")
+            if axes.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+                axes = axes.to(torch.int64).clamp(0, 2**31 - 1)  # int32 would wrap round
             axes = axes.to(torch.int32).contiguous()
         no_tangent_check("Rotary", inv_freq)
         self.requires_grad = inv_freq.requires_grad

@@ -323,3 +323,12 @@ def test_an_infinity_hides_only_itself(cuda, dtype, D, at):
     row = got[0, 1, 2]
     assert torch.isnan(row[at]) and (row[torch.arange(D, device=cuda) != at] == 0).all()
     assert torch.isfinite(got[0, 0]).all() and torch.isfinite(got[0, 1, :2]).all()
+
+
+def test_axes_outside_32_bits_mean_the_nearest(cuda):
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(1, 2, 4, 64, generator=g)
+    pos = torch.randint(0, 500, (3, 4), generator=g)
+    far = torch.tensor([2**32, 2**32 + 1, -2**40, 2**31, -1, 7, 0, 2] * 4)
+    got, _ = norm_rope(x.to(cuda), None, pos.to(cuda), Rotary(freqs(64).to(cuda), axes=far.to(cuda)))
+    check(got, *expect(x, None, ref_angles(pos, freqs(64), far.clamp(0, 2)), F32, norm=False))
