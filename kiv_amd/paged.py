@@ -170,7 +170,7 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
     page is not there is dropped; a slot that two new tokens name holds parts
     of both rows.
     """
-    no_grad_check("paged_append", q, k, v, cache._k, cache._v, rotary, q_norm, k_norm, v_norm, q_out)
+    no_grad_check("paged_append", q, k, v, cache._k, cache._v)
     key = (cache._geometry, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype,
            None if q is None else (q.shape, q.stride(), q.dtype))
     plan = _append_plans.get(key)
@@ -201,6 +201,7 @@ def paged_append(cache: PagedKVCache, batch: PagedBatch, k: torch.Tensor, v: tor
             q_out = torch.empty_like(q)
             args.q_out = q_out.data_ptr()
         else:
+            no_grad_check("paged_append", q_out)
             args.q_out, lay = out_rows(q_out, q, "q_out")
             args.q_out_stride = lay.strides
         if q_norm is not None:
@@ -256,7 +257,7 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
     query or the pages) or a new tensor.  Rows that see no key are zero; rows
     past the last sequence stay as they are (in a new tensor: undefined).
     """
-    no_grad_check("paged_attention", query, cache._k, cache._v, out)
+    no_grad_check("paged_attention", query, cache._k, cache._v)
     dev = cache.device
     if query.device != dev or batch.device != dev:
         raise ValueError(f"query is on {query.device}, the batch on {batch.device}, the cache on {dev}")
@@ -275,6 +276,7 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=dev)
     else:
+        no_grad_check("paged_attention", out)
         out_rows(out, query, "out")
         if not out.is_contiguous():
             raise ValueError("out must be contiguous")

@@ -50,6 +50,8 @@ class HeadNorm:
         return self._weight
 
     def check(self, head_dim: int, device: torch.device) -> nat.HeadNormArgs:
+        if self.requires_grad:
+            no_grad_check("HeadNorm", self)
         at = self._at
         if at is not None and at != (head_dim, device):
             raise ValueError(f"norm weight is [{at[0]}] on {at[1]}, rows have head_dim {head_dim} on {device}")
@@ -109,6 +111,8 @@ class Rotary:
              device: torch.device, batched: bool) -> None:
         """Set the positions in ``dst``: [tokens], [batch, tokens] (``batched``)
         or either behind an axis dimension."""
+        if self.requires_grad:
+            no_grad_check("Rotary", self)
         if self.device != device:
             raise ValueError(f"inv_freq is on {self.device}, rows on {device}")
         lead = self._axes is not None
@@ -154,13 +158,12 @@ def no_grad_check(what: str, *inputs: torch.Tensor | HeadNorm | Rotary | None) -
         for x in inputs:
             if x is not None and x.requires_grad:
                 raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad()")
-    no_tangent_check(what, *inputs)
+    # Tangents exist within a level only; asking each tensor costs 0.3 us.
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        no_tangent_check(what, *inputs)
 
 
 def no_tangent_check(what: str, *inputs: torch.Tensor | HeadNorm | Rotary | None) -> None:
-    # Tangents exist within a level only; asking each tensor costs 0.3 us.
-    if getattr(forward_ad, "_current_level", 0) < 0:
-        return
     for x in inputs:
         if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
             raise RuntimeError(f"{what} has no forward-mode derivative")
@@ -199,7 +202,7 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor |
     fp32, fp16 and bf16; head_dim a multiple of 16 bytes up to 512, the
     rotated width of 32 bytes.  Returns (q_out, k_out).
     """
-    no_grad_check("norm_rope", q, k, rotary, q_norm, k_norm, q_out, k_out)
+    no_grad_check("norm_rope", q, k)
     dev = q.device
     if dev.type != "cuda":
         raise ValueError("norm_rope needs GPU tensors")
@@ -218,6 +221,7 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor |
         q_out = torch.empty_like(q)
         args.q_out = q_out.data_ptr()
     else:
+        no_grad_check("norm_rope", q_out)
         args.q_out, lay = out_rows(q_out, q, "q_out")
         args.q_out_stride = lay.strides
     if q_norm is not None:
@@ -234,6 +238,7 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor |
             k_out = torch.empty_like(k)
             args.k_out = k_out.data_ptr()
         else:
+            no_grad_check("norm_rope", k_out)
             args.k_out, lay = out_rows(k_out, k, "k_out")
             args.k_out_stride = lay.strides
         if k_norm is not None:
