@@ -24,8 +24,8 @@
 //   O^T += V^T P^T: B is the lane's own probabilities (with 16-bit types in
 //   two operands), A the same keys of dim l % 16 from the LDS.
 // Bound: memory (each K and V byte is used by at most 16 rows): 64 sequences
-// of up to 8192 keys, 28 heads over 4 of 128, 97 us (5.3 TB/s); one token over
-// a million keys 359 us (6.0 TB/s); both without the merge.
+// of up to 8192 keys, 28 heads over 4 of 128, 95 us (5.4 TB/s); one token over
+// a million keys 357 us (6.0 TB/s); both without the merge.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -584,9 +584,10 @@ paged_rows_kernel(PagedAttnParams p) {
 // this one, then adds this tile's values beside the next one's maxima, so
 // that vector and matrix instructions alternate in one wave's stream.
 // Bound: neither unit is full (matrix cores busy 51% of the cycles): 4096 tokens
-// over 8192 keys, 12 heads over 2 of 128, 174 to 185 us with the merge, 840 to
-// 890 TFLOP/s; 1 PFLOP/s on long keys.  Two waves a SIMD: the registers hold no
-// third.
+// over 8192 keys, 12 heads over 2 of 128, 338,000 cycles: 168 us at 2.0 GHz, 200
+// after a dozen calls back to back, whose matrix work lowers the clock; a call
+// with the merge 174 to 200 us, 770 to 890 TFLOP/s, 1 PFLOP/s on long keys.  Two
+// waves a SIMD: the registers hold no third.
 template <int KT> struct ChunkGeom {
   static constexpr int D = 32 * KT, CPR = D / 8;
   static constexpr int CP = CPR <= 4 ? 4 : CPR <= 8 ? 8 : CPR <= 16 ? 16 : 32;  // chunks of an LDS row

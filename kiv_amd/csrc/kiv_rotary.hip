@@ -16,11 +16,12 @@
 //
 // Bound: memory (each row read and written once): 4096 tokens of 32 rows of 128
 // bf16 with norms 15.6 us a call, 4.3 TB/s, 86% of a copy's rate; 3856 tokens'
-// K and V rows of 32 heads of 96 into pages 24.9 us, 3.8 TB/s; one token 3.4 us
+// K and V rows of 32 heads of 96 into pages 24.7 us, 3.8 TB/s; one token 3.7 us
 // on the GPU.  A wave has all its rows' loads in flight before it forms the
-// angles; few tokens are dealt a row group a wave, many tokens kRopeBatch row
-// groups a wave, whose angles are then formed once (two groups 16.3 us on the
-// 4096 tokens, eight 18.7, one 15.9; on the pages 25.8, 31.5, 28.2).
+// angles (in the paged form behind the lookup of its sequence and page); few
+// tokens are dealt a row group a wave, many tokens kRopeBatch row groups a wave,
+// whose angles are then formed once (two groups 16.3 us on the 4096 tokens,
+// eight 18.7, one 15.9; on the pages 25.8, 31.5, 28.2).
 #include <climits>
 #include <type_traits>
 
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(RopeParams p) {
   const bool in0 = c0 < p.cpr, in1 = c1 < p.cpr;
   const int e0 = in0 ? c0 : 0, e1 = in1 ? c1 : 0;
 
-  // All loads first.
+  // All rows' loads, then the angles.
   uint4 x0[U], x1[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
